@@ -1,0 +1,434 @@
+// Torch bindings of the dense kernels (dense.h): argument checks, workspaces
+// from torch's allocator, launches on the current stream of x's device.
+#include "layer_bind.h"
+
+#include <vector>
+
+#include "dense.h"
+
+namespace {
+using namespace ngl::dense;
+using namespace ngl::bind;
+
+constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1024;  // tile coordinates are 32-bit
+
+int act_of(const std::string& a) {
+  if (a == "none") return kActNone;
+  if (a == "relu") return kActRelu;
+  if (a == "gelu") return kActGelu;
+  if (a == "gelu_tanh") return kActGeluTanh;
+  if (a == "silu") return kActSilu;
+  TORCH_CHECK(false, "activation must be one of none, relu, gelu, gelu_tanh, silu; got ", a);
+  return -1;
+}
+
+// An operand that TMA can address: itself, or a copy with padded rows.
+Operand tma_operand(const Rows& r, int64_t rows, int64_t cols, std::vector<torch::Tensor>& keep, cudaStream_t s) {
+  const int elem = (int)r.t.element_size();
+  if (reinterpret_cast<uintptr_t>(r.p()) % 16 == 0 && (r.ld * elem) % 16 == 0) return {r.p(), r.ld};
+  const int64_t per = 16 / elem, ldd = (cols + per - 1) / per * per;
+  auto t = torch::empty({rows, ldd}, r.t.options());
+  ck(repack(r.p(), r.ld, t.data_ptr(), ldd, rows, cols, elem, s), "repack");
+  keep.push_back(t);
+  return {t.data_ptr(), ldd};
+}
+
+void run_gemm(Gemm& g, const torch::Tensor& like, std::vector<torch::Tensor>& keep, cudaStream_t s) {
+  const int sms = sm_count(like.get_device());
+  plan(g, sms, true);
+  g.partial = nullptr;
+  if (const int64_t f = partial_floats(g)) {
+    keep.push_back(torch::empty({f}, like.options().dtype(torch::kFloat32)));
+    g.partial = keep.back().data_ptr<float>();
+  }
+  ck(gemm(g, sms, s), "dense product");
+}
+
+struct Shape {
+  int64_t m, k, n;
+};
+// Checks shared by both forms; weights[0] is [n, k].
+Shape check_operands(const torch::Tensor& x, const std::vector<std::pair<torch::Tensor, const char*>>& weights,
+                     const OptTensor& x_scale, const std::vector<std::pair<OptTensor, const char*>>& w_scales) {
+  TORCH_CHECK(x.dim() >= 1, "x needs at least one dimension");
+  const auto t = x.scalar_type();
+  const bool fp8 = t == at::kFloat8_e4m3fn;
+  TORCH_CHECK(fp8 || is_half(t), "x must be bfloat16, float16 or float8_e4m3fn; got ", t);
+  Shape s;
+  s.k = x.size(-1);
+  TORCH_CHECK(s.k > 0, "x has no features (its last dimension is 0)");
+  s.m = x.numel() / s.k;
+  s.n = 0;
+  for (size_t i = 0; i < weights.size(); ++i) {
+    const auto& w = weights[i].first;
+    TORCH_CHECK(w.dim() == 2 && w.size(1) == s.k, weights[i].second, " must be [out_features, ", text(s.k), "]; got ",
+                text(w.sizes()));
+    TORCH_CHECK(w.scalar_type() == t, weights[i].second, " must be ", t, " like x; got ", w.scalar_type());
+    if (i == 0) s.n = w.size(0);
+    TORCH_CHECK(w.size(0) == s.n, "the two projections must have the same out_features; got ", text(s.n), " and ",
+                text(w.size(0)));
+  }
+  TORCH_CHECK(s.m <= kMaxDim && s.n <= kMaxDim && s.k <= kMaxDim, "a dimension exceeds ", text(kMaxDim));
+  TORCH_CHECK(fp8 == x_scale.has_value(), fp8 ? "8-bit x needs x_scale" : "x_scale needs an 8-bit x");
+  if (fp8)
+    TORCH_CHECK(x_scale->scalar_type() == torch::kFloat32 && x_scale->numel() == s.m,
+                "x_scale must be float32 with one value a row (", text(s.m), "); got ", text(x_scale->sizes()));
+  for (const auto& ws : w_scales) {
+    TORCH_CHECK(fp8 == ws.first.has_value(), ws.second, fp8 ? " is needed with 8-bit weights" : " needs 8-bit weights");
+    if (fp8)
+      TORCH_CHECK(ws.first->scalar_type() == torch::kFloat32 && ws.first->numel() == s.n, ws.second,
+                  " must be float32 with one value an output feature (", text(s.n), "); got ", text(ws.first->sizes()));
+  }
+  return s;
+}
+
+std::vector<int64_t> out_shape(const torch::Tensor& x, int64_t n) {
+  auto v = x.sizes().vec();
+  v.back() = n;
+  return v;
+}
+
+Epilogue empty_epilogue() {
+  Epilogue e;
+  std::memset(&e, 0, sizeof(e));
+  return e;
+}
+
+// y, z (z undefined unless keep_z).
+std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight, OptTensor bias, OptTensor residual,
+                                          const std::string& activation, OptTensor x_scale, OptTensor w_scale,
+                                          c10::optional<at::ScalarType> out_dtype, bool keep_z) {
+  const int act = act_of(activation);
+  const Shape sh = check_operands(x, {{weight, "weight"}}, x_scale, {{w_scale, "w_scale"}});
+  const bool fp8 = x.scalar_type() == at::kFloat8_e4m3fn;
+  auto half = fp8 ? torch::kBFloat16 : x.scalar_type();
+  if (fp8 && out_dtype.has_value() && is_half(*out_dtype)) half = *out_dtype;
+  if (fp8 && bias.has_value() && is_half(bias->scalar_type()) && !(out_dtype.has_value() && is_half(*out_dtype)))
+    half = bias->scalar_type();
+  auto out_t = half;
+  if (residual.has_value()) {
+    if (fp8 && !out_dtype.has_value() && !bias.has_value() && is_half(residual->scalar_type()))
+      half = residual->scalar_type();
+    out_t = residual->scalar_type();
+    TORCH_CHECK(out_t == half || out_t == torch::kFloat32, "residual must be ", half, " or float32; got ", out_t);
+    TORCH_CHECK(residual->sizes().vec() == out_shape(x, sh.n), "residual must have the output's shape ",
+                text(out_shape(x, sh.n)), "; got ", text(residual->sizes()));
+  }
+  if (out_dtype.has_value()) {
+    TORCH_CHECK(*out_dtype == half || *out_dtype == torch::kFloat32, "out_dtype must be ", half, " or float32; got ",
+                *out_dtype);
+    TORCH_CHECK(!residual.has_value() || out_t == *out_dtype, "the output has the residual's type ", out_t,
+                ", not out_dtype ", *out_dtype);
+    out_t = *out_dtype;
+  }
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == sh.n, "bias must be [", text(sh.n), "]; got ", text(bias->sizes()));
+    TORCH_CHECK(bias->scalar_type() == half, "bias must be ", half, "; got ", bias->scalar_type());
+  }
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
+  need_cuda(weight, x, "weight");
+  if (bias.has_value()) need_cuda(*bias, x, "bias");
+  if (residual.has_value()) need_cuda(*residual, x, "residual");
+  if (fp8) {
+    need_cuda(*x_scale, x, "x_scale");
+    need_cuda(*w_scale, x, "w_scale");
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  cudaStream_t s = at::cuda::getCurrentCUDAStream();
+  auto y = torch::empty(out_shape(x, sh.n), x.options().dtype(out_t));
+  torch::Tensor z;
+  if (keep_z) z = torch::empty({sh.m, sh.n}, x.options().dtype(half));
+  if (y.numel() == 0) return {y, z};
+
+  std::vector<torch::Tensor> keep;
+  const Rows xr = rows_of(x, sh.m, sh.k), wr = rows_of(weight, sh.n, sh.k);
+  Epilogue ep = empty_epilogue();
+  ep.act = act;
+  ep.half_type = type_of(half);
+  ep.out_type = type_of(out_t);
+  ep.out[0] = y.data_ptr();
+  ep.ldo = sh.n;
+  if (keep_z) ep.z[0] = z.data_ptr();
+  if (bias.has_value()) {
+    keep.push_back(bias->contiguous());
+    ep.bias = keep.back().data_ptr();
+  }
+  if (residual.has_value()) {
+    const Rows rr = rows_of(*residual, sh.m, sh.n);
+    keep.push_back(rr.t);
+    ep.residual = rr.p();
+    ep.ldr = rr.ld;
+  }
+  if (fp8) {
+    keep.push_back(x_scale->contiguous());
+    ep.row_scale = keep.back().data_ptr<float>();
+    keep.push_back(w_scale->contiguous());
+    ep.col_scale[0] = keep.back().data_ptr<float>();
+  }
+  if (sh.m <= kSkinnyRows) {
+    Skinny g;
+    std::memset(&g, 0, sizeof(g));
+    g.m = sh.m, g.n = sh.n, g.k = sh.k;
+    g.type = type_of(x.scalar_type());
+    g.x = {xr.p(), xr.ld};
+    g.w[0] = {wr.p(), wr.ld};
+    g.ep = ep;
+    ck(skinny(g, s), "linear");
+    return {y, z};
+  }
+  Gemm g;
+  std::memset(&g, 0, sizeof(g));
+  g.m = sh.m, g.n = sh.n, g.k = sh.k;
+  g.type = type_of(x.scalar_type());
+  g.major_a = g.major_b = kMajorK;
+  g.dual = kDualNone;
+  g.a[0] = tma_operand(xr, sh.m, sh.k, keep, s);
+  g.b[0] = tma_operand(wr, sh.n, sh.k, keep, s);
+  g.ep = ep;
+  run_gemm(g, x, keep, s);
+  return {y, z};
+}
+
+// out [m, n] of like's type = A B^T with the given orders; plain epilogue.
+void plain_product(Gemm& g, std::vector<torch::Tensor> outs, const torch::Tensor& like,
+                   std::vector<torch::Tensor>& keep, cudaStream_t s) {
+  g.type = type_of(like.scalar_type());
+  g.ep = empty_epilogue();
+  g.ep.half_type = g.ep.out_type = g.type;
+  g.ep.ldo = g.n;
+  for (size_t i = 0; i < outs.size(); ++i) g.ep.out[i] = outs[i].data_ptr();
+  run_gemm(g, like, keep, s);
+}
+
+// dx, dw, db (undefined where not needed).
+std::vector<torch::Tensor> linear_backward(torch::Tensor dy, torch::Tensor x, torch::Tensor weight, OptTensor z,
+                                           const std::string& activation, bool need_x, bool need_w, bool need_b) {
+  const int act = act_of(activation);
+  const Shape sh = check_operands(x, {{weight, "weight"}}, c10::nullopt, {});
+  TORCH_CHECK(is_half(x.scalar_type()), "no gradient through 8-bit operands");
+  TORCH_CHECK(dy.sizes().vec() == out_shape(x, sh.n), "gradient must have the output's shape");
+  TORCH_CHECK(dy.scalar_type() == x.scalar_type() || dy.scalar_type() == torch::kFloat32,
+              "gradient must be ", x.scalar_type(), " or float32; got ", dy.scalar_type());
+  TORCH_CHECK(act == kActNone || z.has_value(), "the activation's gradient needs z");
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
+  need_cuda(dy, x, "gradient");
+  need_cuda(weight, x, "weight");
+  const c10::cuda::CUDAGuard guard(x.device());
+  cudaStream_t s = at::cuda::getCurrentCUDAStream();
+  torch::Tensor dx, dw, db;
+  if (sh.m == 0 || sh.n == 0) {
+    if (need_x) dx = torch::zeros_like(x);
+    if (need_w) dw = torch::zeros({sh.n, sh.k}, weight.options());
+    if (need_b) db = torch::zeros({sh.n}, weight.options());
+    return {dx, dw, db};
+  }
+  std::vector<torch::Tensor> keep;
+  const int half = type_of(x.scalar_type());
+  Rows dzr = rows_of(dy, sh.m, sh.n);
+  const bool make_dz = act != kActNone || dy.scalar_type() != x.scalar_type();
+  if (need_b || (make_dz && (need_x || need_w))) {
+    torch::Tensor dz, part;
+    if (make_dz && (need_x || need_w)) dz = torch::empty({sh.m, sh.n}, x.options());
+    const int parts = colsum_parts(sh.m, sh.n, sm_count(x.get_device()));
+    if (need_b) {
+      db = torch::empty({sh.n}, x.options());
+      part = torch::empty({parts, sh.n}, x.options().dtype(torch::kFloat32));
+    }
+    ck(act_backward(dzr.p(), type_of(dy.scalar_type()), dzr.ld, act != kActNone ? z->data_ptr() : nullptr, act, half,
+                    sh.m, sh.n, dz.defined() ? dz.data_ptr() : nullptr, need_b ? part.data_ptr<float>() : nullptr,
+                    parts, need_b ? db.data_ptr() : nullptr, s),
+       "activation gradient");
+    keep.push_back(dzr.t);
+    if (dz.defined()) dzr = {dz, sh.n};
+  }
+  if (!need_x && !need_w) return {dx, dw, db};
+  const Operand dz = tma_operand(dzr, sh.m, sh.n, keep, s);
+  if (need_x) {
+    dx = torch::empty(x.sizes(), x.options());
+    Gemm g;
+    std::memset(&g, 0, sizeof(g));
+    g.m = sh.m, g.n = sh.k, g.k = sh.n;
+    g.major_a = kMajorK, g.major_b = kMajorMN;
+    g.a[0] = dz;
+    g.b[0] = tma_operand(rows_of(weight, sh.n, sh.k), sh.n, sh.k, keep, s);
+    plain_product(g, {dx}, x, keep, s);
+  }
+  if (need_w) {
+    dw = torch::empty({sh.n, sh.k}, weight.options());
+    Gemm g;
+    std::memset(&g, 0, sizeof(g));
+    g.m = sh.n, g.n = sh.k, g.k = sh.m;
+    g.major_a = g.major_b = kMajorMN;
+    g.a[0] = dz;
+    g.b[0] = tma_operand(rows_of(x, sh.m, sh.k), sh.m, sh.k, keep, s);
+    plain_product(g, {dw}, x, keep, s);
+  }
+  return {dx, dw, db};
+}
+
+// h, g, u (g and u undefined unless keep).
+std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
+                                         const std::string& activation, OptTensor x_scale, OptTensor gate_scale,
+                                         OptTensor up_scale, c10::optional<at::ScalarType> out_dtype, bool keep_zs) {
+  const int act = act_of(activation);
+  const Shape sh = check_operands(x, {{w_gate, "w_gate"}, {w_up, "w_up"}}, x_scale,
+                                  {{gate_scale, "gate_scale"}, {up_scale, "up_scale"}});
+  const bool fp8 = x.scalar_type() == at::kFloat8_e4m3fn;
+  auto half = fp8 ? torch::kBFloat16 : x.scalar_type();
+  if (fp8 && out_dtype.has_value() && is_half(*out_dtype)) half = *out_dtype;
+  auto out_t = half;
+  if (out_dtype.has_value()) {
+    TORCH_CHECK(*out_dtype == half || *out_dtype == torch::kFloat32, "out_dtype must be ", half, " or float32; got ",
+                *out_dtype);
+    out_t = *out_dtype;
+  }
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
+  need_cuda(w_gate, x, "w_gate");
+  need_cuda(w_up, x, "w_up");
+  if (fp8) {
+    need_cuda(*x_scale, x, "x_scale");
+    need_cuda(*gate_scale, x, "gate_scale");
+    need_cuda(*up_scale, x, "up_scale");
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  cudaStream_t s = at::cuda::getCurrentCUDAStream();
+  auto h = torch::empty(out_shape(x, sh.n), x.options().dtype(out_t));
+  torch::Tensor zg, zu;
+  if (keep_zs) {
+    zg = torch::empty({sh.m, sh.n}, x.options().dtype(half));
+    zu = torch::empty({sh.m, sh.n}, x.options().dtype(half));
+  }
+  if (h.numel() == 0) return {h, zg, zu};
+  std::vector<torch::Tensor> keep;
+  const Rows xr = rows_of(x, sh.m, sh.k), gr = rows_of(w_gate, sh.n, sh.k), ur = rows_of(w_up, sh.n, sh.k);
+  Epilogue ep = empty_epilogue();
+  ep.act = act;
+  ep.half_type = type_of(half);
+  ep.out_type = type_of(out_t);
+  ep.out[0] = h.data_ptr();
+  ep.ldo = sh.n;
+  if (keep_zs) {
+    ep.z[0] = zg.data_ptr();
+    ep.z[1] = zu.data_ptr();
+  }
+  if (fp8) {
+    keep.push_back(x_scale->contiguous());
+    ep.row_scale = keep.back().data_ptr<float>();
+    keep.push_back(gate_scale->contiguous());
+    ep.col_scale[0] = keep.back().data_ptr<float>();
+    keep.push_back(up_scale->contiguous());
+    ep.col_scale[1] = keep.back().data_ptr<float>();
+  }
+  if (sh.m <= kSkinnyRows) {
+    Skinny g;
+    std::memset(&g, 0, sizeof(g));
+    g.m = sh.m, g.n = sh.n, g.k = sh.k;
+    g.type = type_of(x.scalar_type());
+    g.gated = true;
+    g.x = {xr.p(), xr.ld};
+    g.w[0] = {gr.p(), gr.ld};
+    g.w[1] = {ur.p(), ur.ld};
+    g.ep = ep;
+    ck(skinny(g, s), "gated linear");
+    return {h, zg, zu};
+  }
+  Gemm g;
+  std::memset(&g, 0, sizeof(g));
+  g.m = sh.m, g.n = sh.n, g.k = sh.k;
+  g.type = type_of(x.scalar_type());
+  g.major_a = g.major_b = kMajorK;
+  g.dual = kDualN;
+  g.a[0] = tma_operand(xr, sh.m, sh.k, keep, s);
+  g.b[0] = tma_operand(gr, sh.n, sh.k, keep, s);
+  g.b[1] = tma_operand(ur, sh.n, sh.k, keep, s);
+  g.ep = ep;
+  run_gemm(g, x, keep, s);
+  return {h, zg, zu};
+}
+
+// dx, dw_gate, dw_up (undefined where not needed).
+std::vector<torch::Tensor> gated_backward_(torch::Tensor dh, torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
+                                           torch::Tensor zg, torch::Tensor zu, const std::string& activation,
+                                           bool need_x, bool need_w) {
+  const int act = act_of(activation);
+  const Shape sh = check_operands(x, {{w_gate, "w_gate"}, {w_up, "w_up"}}, c10::nullopt, {});
+  TORCH_CHECK(is_half(x.scalar_type()), "no gradient through 8-bit operands");
+  TORCH_CHECK(dh.sizes().vec() == out_shape(x, sh.n), "gradient must have the output's shape");
+  TORCH_CHECK(dh.scalar_type() == x.scalar_type(), "gradient must be ", x.scalar_type(), "; got ", dh.scalar_type());
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
+  need_cuda(dh, x, "gradient");
+  const c10::cuda::CUDAGuard guard(x.device());
+  cudaStream_t s = at::cuda::getCurrentCUDAStream();
+  torch::Tensor dx, dwg, dwu;
+  if (sh.m == 0 || sh.n == 0) {
+    if (need_x) dx = torch::zeros_like(x);
+    if (need_w) {
+      dwg = torch::zeros({sh.n, sh.k}, w_gate.options());
+      dwu = torch::zeros({sh.n, sh.k}, w_up.options());
+    }
+    return {dx, dwg, dwu};
+  }
+  std::vector<torch::Tensor> keep;
+  const Rows dhr = rows_of(dh, sh.m, sh.n);
+  auto dg = torch::empty({sh.m, sh.n}, x.options()), du = torch::empty({sh.m, sh.n}, x.options());
+  ck(gated_backward(dhr.p(), dhr.ld, zg.data_ptr(), zu.data_ptr(), act, type_of(x.scalar_type()), sh.m, sh.n,
+                    dg.data_ptr(), du.data_ptr(), s),
+     "gate gradient");
+  const Operand og = tma_operand({dg, sh.n}, sh.m, sh.n, keep, s), ou = tma_operand({du, sh.n}, sh.m, sh.n, keep, s);
+  if (need_x) {
+    dx = torch::empty(x.sizes(), x.options());
+    Gemm g;
+    std::memset(&g, 0, sizeof(g));
+    g.m = sh.m, g.n = sh.k, g.k = sh.n;
+    g.major_a = kMajorK, g.major_b = kMajorMN;
+    g.dual = kDualK;
+    g.a[0] = og;
+    g.a[1] = ou;
+    g.b[0] = tma_operand(rows_of(w_gate, sh.n, sh.k), sh.n, sh.k, keep, s);
+    g.b[1] = tma_operand(rows_of(w_up, sh.n, sh.k), sh.n, sh.k, keep, s);
+    plain_product(g, {dx}, x, keep, s);
+  }
+  if (need_w) {
+    dwg = torch::empty({sh.n, sh.k}, w_gate.options());
+    dwu = torch::empty({sh.n, sh.k}, w_up.options());
+    Gemm g;
+    std::memset(&g, 0, sizeof(g));
+    g.m = sh.n, g.n = sh.k, g.k = sh.m;
+    g.major_a = g.major_b = kMajorMN;
+    g.dual = kDualM;
+    g.a[0] = og;
+    g.a[1] = ou;
+    g.b[0] = tma_operand(rows_of(x, sh.m, sh.k), sh.m, sh.k, keep, s);
+    plain_product(g, {dwg, dwu}, x, keep, s);
+  }
+  return {dx, dwg, dwu};
+}
+
+// (CTAs of a tile, accumulator columns, splits of k) that a product of these
+// sizes takes on `sms` SMs.
+std::vector<int64_t> dense_plan(int64_t m, int64_t n, int64_t k, int64_t dual, bool fp8, int64_t sms) {
+  TORCH_CHECK(m > 0 && n > 0 && k > 0 && sms > 1 && dual >= 0 && dual <= 3, "sizes must be positive, dual 0 to 3");
+  Gemm g;
+  std::memset(&g, 0, sizeof(g));
+  g.m = m, g.n = n, g.k = k, g.dual = (int)dual, g.type = fp8 ? kE4M3 : kBF16;
+  plan(g, (int)sms, true);
+  return {g.cg, g.nb, g.splits};
+}
+
+std::vector<int64_t> dense_status(int64_t device, bool clear) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  int v[4] = {0, 0, 0, 0};
+  ck(read_status(v, clear, at::cuda::getCurrentCUDAStream()), "dense status");
+  return {v[0], v[1], v[2], v[3]};
+}
+
+}  // namespace
+
+void register_dense(pybind11::module& m) {
+  m.def("linear_forward", &linear_forward);
+  m.def("linear_backward", &linear_backward);
+  m.def("gated_forward", &gated_forward);
+  m.def("gated_backward", &gated_backward_);
+  m.def("dense_plan", &dense_plan);
+  m.def("dense_status", &dense_status);
+}

@@ -1,0 +1,636 @@
+// Matrix products on the tensor cores with the epilogues of a dense layer.
+//
+// Mathematics: D[i, j] = sum_k A[i, k] B[j, k] for 16-bit or e4m3 operands,
+// sums in fp32, followed by the epilogue of dense.h in the same kernel.  One
+// kernel serves the forward product (both operands with k contiguous), the
+// gradient of the input (B stored as [k, j]) and the gradient of the weight
+// (both stored with k as the slow axis): tcgen05.mma reads either order from
+// shared memory, so no operand is transposed in memory.
+//
+// Layout: persistent CTAs, one per SM (or pairs on one tile).  Warp 0 moves
+// 128-byte-wide tiles with TMA, warp 1 issues the products of 128-byte k
+// blocks, warps 4-11 take finished accumulators from tensor memory through
+// the epilogue while the next tile's products run into the other half of
+// tensor memory.
+#include "dense.h"
+
+#include <algorithm>
+#include <cstring>
+
+#include "dense_math.cuh"
+#include "ngl_cuda.cuh"
+
+namespace ngl {
+namespace dense {
+namespace {
+
+using namespace ngl::dev;
+
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
+constexpr int kRowsA = 128;       // A rows of one CTA
+constexpr int kBlockBytes = 128;  // bytes of k in one stage
+constexpr uint64_t kWaitNs = 4000000000ull;
+constexpr uint64_t kDrainNs = 100000000ull;
+
+__device__ int g_status[4];
+
+struct alignas(64) Maps {
+  CUtensorMap a[2], b[2];
+};
+struct Args {
+  int64_t m, n;
+  int mt, nt;        // tiles of one problem along m and n
+  int kb;            // k blocks of one operand pair
+  int dual, splits;
+  uint32_t idesc;
+  int64_t part_stride;  // floats of one split's partial
+  float* partial;
+  Epilogue ep;
+};
+
+// ------------------------------------------------------------------- PTX
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+  if (try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (!try_wait_cluster(bar, parity))
+    if (globaltimer() - t0 > limit_ns) return false;
+  return true;
+}
+template <int CG>
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+  if (CG == 1)
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, 0))
+                 : "memory");
+}
+// A box of a 2-D tensor map into this CTA's shared memory; the bytes are
+// counted by the pair's first CTA.
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, "
+        "{%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
+  if (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+  if (CG == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+}
+template <int CG, bool kFp8>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+#define NGL_MMA(group, kind)                                                                                       \
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::" group ".kind::" kind           \
+               " [%0], %1, %2, %3, p;\n}\n" ::"r"(d),                                                              \
+               "l"(a), "l"(b), "r"(idesc), "r"(accumulate)                                                         \
+               : "memory")
+  if (CG == 1) {
+    if (kFp8) NGL_MMA("1", "f8f6f4"); else NGL_MMA("1", "f16");
+  } else {
+    if (kFp8) NGL_MMA("2", "f8f6f4"); else NGL_MMA("2", "f16");
+  }
+#undef NGL_MMA
+}
+// Arrive on `bar` (in both CTAs of a pair) once this thread's products are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle.  A tile with k contiguous
+// has groups of 8 rows 1024 bytes apart; a tile with rows contiguous holds
+// chunks of 64 rows of 8192 bytes (64 k of 128 bytes each), 8 k 1024 bytes
+// apart.
+template <int kMaj>
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+  constexpr uint64_t lead = kMaj == kMajorK ? 1 : (8192 >> 4);
+  return (uint64_t)((addr >> 4) & 0x3fff) | (lead << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Bytes from one product's k to the next inside a stage (32 bytes of k).
+template <int kMaj>
+constexpr uint32_t kStep = kMaj == kMajorK ? 32u : 2048u;
+
+template <int CG, int NB>
+struct Shape {
+  static constexpr int kRowsB = NB / CG;  // B rows of one CTA
+  static constexpr int kBytesA = kRowsA * kBlockBytes;
+  static constexpr int kBytesB = kRowsB * kBlockBytes;
+  static constexpr int kStage = kBytesA + kBytesB;
+  static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
+  static constexpr int kCols = 2 * NB;  // tensor memory: two accumulators
+  static constexpr int kSmem = kStages * kStage + 1024 /* alignment */ + 256 /* barriers */;
+};
+
+struct Item {
+  int prob;     // kDualM: which product
+  int mt, nt;   // tile
+  int split;
+  int k0, k1;   // k blocks
+};
+// Work item w.  Groups of 8 rows of tiles sweep the columns together, so that
+// the tiles that run at one time share their operands in L2.
+__device__ __forceinline__ Item item_of(const Args& g, int64_t w) {
+  const int rows = g.mt * (g.dual == kDualM ? 2 : 1);
+  const int64_t tiles = (int64_t)rows * g.nt;
+  Item it;
+  it.split = (int)(w / tiles);
+  const int64_t t = w - it.split * tiles;
+  const int per = 8 * g.nt;
+  const int grp = (int)(t / per), in = (int)(t - (int64_t)grp * per);
+  const int h = min(8, rows - grp * 8);
+  it.nt = in / h;
+  const int r = grp * 8 + in % h;
+  it.prob = r / g.mt;
+  it.mt = r - it.prob * g.mt;
+  const int kb = g.kb * (g.dual == kDualK ? 2 : 1);
+  it.k0 = (int)((int64_t)kb * it.split / g.splits);
+  it.k1 = (int)((int64_t)kb * (it.split + 1) / g.splits);
+  return it;
+}
+
+template <int CG, int NB, int MA, int MB, bool kFp8, bool kGated>
+__global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+  using S = Shape<CG, NB>;
+  constexpr int kBk = kFp8 ? 128 : 64;  // k of one stage
+  constexpr int kTileN = kGated ? NB / 2 : NB;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = base + S::kStages * S::kStage;
+  auto full = [&](int s) { return bars + 8u * s; };
+  auto empty = [&](int s) { return bars + 8u * (S::kStages + s); };
+  auto tfull = [&](int b) { return bars + 8u * (2 * S::kStages + b); };
+  auto tempty = [&](int b) { return bars + 8u * (2 * S::kStages + 2 + b); };
+  const uint32_t drained = bars + 8u * (2 * S::kStages + 4);
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cta_rank() : 0u;
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int s = 0; s < S::kStages; ++s) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full(s)) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty(s)) : "memory");
+    }
+    for (int b = 0; b < 2; ++b) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(tfull(b)) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tempty(b)), "r"(CG * kEpiWarps) : "memory");
+    }
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(drained) : "memory");
+    fence_mbar_init();
+  }
+  if (warp == 2) tmem_alloc<CG>(smem_u32(&tmem_base_s), S::kCols);
+  fence_before();
+  if (CG == 2) cluster_sync(); else __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_base_s;
+
+  const int64_t items = (int64_t)g.mt * (g.dual == kDualM ? 2 : 1) * g.nt * g.splits;
+  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  volatile int* const aborted = &abort_s;
+
+  if (warp == 0 && lane == 0) {
+    // ---- loads
+    int s = 0;
+    uint32_t ph = 0;
+    int64_t loads = 0;
+    bool ok = true;
+    for (int64_t w = first; ok && w < items; w += step) {
+      const Item it = item_of(g, w);
+      const int row_a = (it.mt * CG + (int)rank) * kRowsA;
+      for (int kb = it.k0; kb < it.k1; ++kb) {
+        if (*aborted || !wait_bar(empty(s), ph ^ 1u, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        if (rank == 0) mbar_expect_tx(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(full(s))), CG * S::kStage);
+        const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
+        const int seg = g.dual == kDualK && kb >= g.kb ? 1 : 0;
+        const int k = (kb - seg * g.kb) * kBk;
+        const CUtensorMap* ma = &maps.a[g.dual == kDualM ? it.prob : seg];
+        const uint32_t da = base + s * S::kStage, db = da + S::kBytesA;
+        if (MA == kMajorK) {
+          tma_load<CG>(da, ma, k, row_a, bar);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kRowsA / 64; ++c) tma_load<CG>(da + c * 8192, ma, row_a + 64 * c, k, bar);
+        }
+        if (kGated) {
+          // gate rows in the accumulator's first half, up rows in its second
+          if (CG == 2) {
+            tma_load<CG>(db, &maps.b[rank], k, it.nt * kTileN, bar);
+          } else {
+            tma_load<CG>(db, &maps.b[0], k, it.nt * kTileN, bar);
+            tma_load<CG>(db + S::kBytesB / 2, &maps.b[1], k, it.nt * kTileN, bar);
+          }
+        } else {
+          const CUtensorMap* mb = &maps.b[seg];
+          const int row_b = it.nt * NB + (int)rank * S::kRowsB;
+          if (MB == kMajorK) {
+            tma_load<CG>(db, mb, k, row_b, bar);
+          } else {
+#pragma unroll
+            for (int c = 0; c < S::kRowsB / 64; ++c) tma_load<CG>(db + c * 8192, mb, row_b + 64 * c, k, bar);
+          }
+        }
+        ++loads;
+        if (++s == S::kStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    if (!ok) {
+      *aborted = 1;
+      set_status(g_status, kTimeoutCopy, (int)blockIdx.x, 0);
+      // copies in flight land before the shared memory is given up
+      if (rank == 0) {
+        const int64_t from = loads > S::kStages ? loads - S::kStages : 0;
+        for (int64_t l = from; l < loads; ++l)
+          wait_bar(full((int)(l % S::kStages)), (uint32_t)((l / S::kStages) & 1), kDrainNs);
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---- products
+    int s = 0;
+    uint32_t ph = 0;
+    int buf = 0;
+    uint32_t bph = 0;
+    bool ok = true;
+    for (int64_t w = first; ok && w < items; w += step) {
+      const Item it = item_of(g, w);
+      if (*aborted || !wait_bar(tempty(buf), bph ^ 1u, kWaitNs)) {
+        ok = false;
+        break;
+      }
+      fence_after();
+      const uint32_t d = tmem + buf * NB;
+      for (int kb = it.k0; kb < it.k1; ++kb) {
+        if (!wait_bar(full(s), ph, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        const uint32_t sa = base + s * S::kStage, sb = sa + S::kBytesA;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma<CG, kFp8>(d, smem_desc<MA>(sa + j * kStep<MA>), smem_desc<MB>(sb + j * kStep<MB>), g.idesc,
+                        (kb > it.k0 || j > 0) ? 1u : 0u);
+        commit<CG>(empty(s));
+        if (++s == S::kStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+      }
+      commit<CG>(tfull(buf));
+      if (++buf == 2) {
+        buf = 0;
+        bph ^= 1u;
+      }
+    }
+    if (!ok) {
+      *aborted = 1;
+      set_status(g_status, kTimeoutPayload, (int)blockIdx.x, 1);
+      commit<CG>(drained);
+      wait_bar(drained, 0, kDrainNs);
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue
+    const int quad = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    const EpiVec ev = epi_vec(g.ep, g.n);
+    int buf = 0;
+    uint32_t bph = 0;
+    for (int64_t w = first; w < items; w += step) {
+      const Item it = item_of(g, w);
+      if (*aborted || !wait_bar(tfull(buf), bph, kWaitNs)) {
+        *aborted = 1;
+        if (lane == 0) set_status(g_status, kTimeoutResult, (int)blockIdx.x, 2);
+        break;
+      }
+      __syncwarp();
+      fence_after();
+      const int64_t row = (int64_t)(it.mt * CG + (int)rank) * kRowsA + quad * 32 + lane;
+      const bool inside = row < g.m;
+      const uint32_t acc = lanes + buf * NB;
+      const int64_t col0 = (int64_t)it.nt * kTileN;
+      if (kGated) {
+#pragma unroll 1
+        for (int c = half * (kTileN / 2); c < (half + 1) * (kTileN / 2); c += 32) {
+          float v[32], u[32];
+          tmem_load32(acc + c, v);
+          tmem_load32(acc + kTileN + c, u);
+          tmem_load_wait();
+          if (!inside || col0 + c >= g.n) continue;
+          if (g.splits > 1) {
+            const int valid = (int)min64(32, g.n - col0 - c);
+            const bool vec = g.n % 4 == 0;
+            float* p = g.partial + it.split * g.part_stride;
+            put_run<32>(p, row * g.n + col0 + c, kF32, valid, vec, v);
+            put_run<32>(p + g.m * g.n, row * g.n + col0 + c, kF32, valid, vec && (g.m * g.n) % 4 == 0, u);
+          } else {
+            epilogue_gated_run<32>(g.ep, ev, row, col0 + c, g.n, v, u);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = half * (NB / 2); c < (half + 1) * (NB / 2); c += 32) {
+          float v[32];
+          tmem_load32(acc + c, v);
+          tmem_load_wait();
+          if (!inside || col0 + c >= g.n) continue;
+          if (g.splits > 1) {
+            float* p = g.partial + it.split * g.part_stride + it.prob * g.m * g.n;
+            put_run<32>(p, row * g.n + col0 + c, kF32, (int)min64(32, g.n - col0 - c),
+                        g.n % 4 == 0 && (g.m * g.n) % 4 == 0, v);
+          } else {
+            epilogue_run<32>(g.ep, ev, it.prob, row, col0 + c, g.n, v);
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_leader<CG>(tempty(buf));
+      if (++buf == 2) {
+        buf = 0;
+        bph ^= 1u;
+      }
+    }
+  }
+  __syncwarp();
+  fence_before();
+  if (CG == 2) cluster_sync(); else __syncthreads();
+  fence_after();
+  if (warp == 2) tmem_free<CG>(tmem, S::kCols);
+}
+
+// Sum of the splits in their order, then the epilogue.  One thread takes 8
+// columns of one row.
+template <bool kGated>
+__global__ void __launch_bounds__(256) k_join(Args g) {
+  const int64_t nc = (g.n + 7) / 8;
+  const int probs = g.dual == kDualM ? 2 : 1;
+  const EpiVec ev = epi_vec(g.ep, g.n);
+  const bool vec = g.n % 4 == 0 && (g.m * g.n) % 4 == 0;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < nc * g.m * probs;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int prob = (int)(i / (nc * g.m));
+    const int64_t r = i - prob * nc * g.m, row = r / nc, col = (r - row * nc) * 8;
+    const int valid = (int)min64(8, g.n - col);
+    float v[8] = {}, u[8] = {};
+    for (int s = 0; s < g.splits; ++s) {
+      const float* p = g.partial + s * g.part_stride + prob * g.m * g.n;
+      float t[8];
+      get_run<8>(p, row * g.n + col, kF32, valid, vec, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += t[j];
+      if (kGated) {
+        get_run<8>(p + g.m * g.n, row * g.n + col, kF32, valid, vec, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] += t[j];
+      }
+    }
+    if (kGated)
+      epilogue_gated_run<8>(g.ep, ev, row, col, g.n, v, u);
+    else
+      epilogue_run<8>(g.ep, ev, prob, row, col, g.n, v);
+  }
+}
+
+// ------------------------------------------------------------------ host
+// The driver's tensor-map encoder, found at run time: the library loads on
+// machines without a driver (builds, CPU tests).
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
+bool make_map(CUtensorMap* map, const Operand& o, int type, int major, int64_t rows, int64_t k, int box_rows) {
+  const int elem = type_bytes(type);
+  const cuuint64_t dims[2] = {(cuuint64_t)(major == kMajorK ? k : rows), (cuuint64_t)(major == kMajorK ? rows : k)};
+  const cuuint64_t strides[1] = {(cuuint64_t)(o.ld * elem)};
+  const cuuint32_t box[2] = {(cuuint32_t)(kBlockBytes / elem), (cuuint32_t)(major == kMajorK ? box_rows : 64)};
+  const cuuint32_t es[2] = {1, 1};
+  const CUtensorMapDataType dt = type == kBF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : type == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const EncodeFn encode = encoder();
+  return encode(map, dt, 2, const_cast<void*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Instruction descriptor: fp32 sums, operand types and orders, tile size.
+uint32_t make_idesc(const Gemm& g) {
+  const uint32_t t = g.type == kBF16 ? 1u : 0u;  // f16 and e4m3 are both 0 in their kinds
+  return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)(g.major_a == kMajorMN) << 15) |
+         ((uint32_t)(g.major_b == kMajorMN) << 16) | ((uint32_t)(g.nb / 8) << 17) | ((uint32_t)(128 * g.cg / 16) << 24);
+}
+
+template <int CG, int NB, int MA, int MB, bool kFp8, bool kGated>
+cudaError_t launch(const Maps& maps, const Args& args, int sms, cudaStream_t s) {
+  using S = Shape<CG, NB>;
+  auto* fn = &k_gemm<CG, NB, MA, MB, kFp8, kGated>;
+  // once a device; setting it again is harmless
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t items = (int64_t)args.mt * (args.dual == kDualM ? 2 : 1) * args.nt * args.splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(items, sms / CG)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, maps, args);
+}
+
+template <int MA, int MB, bool kFp8, bool kGated>
+cudaError_t launch_shape(const Gemm& g, const Maps& maps, const Args& args, int sms, cudaStream_t s) {
+  if (g.cg == 2)
+    return g.nb == 256 ? launch<2, 256, MA, MB, kFp8, kGated>(maps, args, sms, s)
+                       : launch<2, 128, MA, MB, kFp8, kGated>(maps, args, sms, s);
+  return g.nb == 256 ? launch<1, 256, MA, MB, kFp8, kGated>(maps, args, sms, s)
+                     : launch<1, 128, MA, MB, kFp8, kGated>(maps, args, sms, s);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+}  // namespace
+
+int64_t partial_floats(const Gemm& g) {
+  return g.splits > 1 ? (int64_t)g.splits * g.m * g.n * (g.dual == kDualN || g.dual == kDualM ? 2 : 1) : 0;
+}
+
+void plan(Gemm& g, int sms, bool may_split) {
+  const int bk = g.type == kE4M3 ? 128 : 64;
+  const int64_t kb = ceil_div(g.k, bk) * (g.dual == kDualK ? 2 : 1);
+  double best = 1e30;
+  for (int cg = 1; cg <= 2; ++cg)
+    for (int nb = 128; nb <= 256; nb += 128) {
+      const int64_t tn = g.dual == kDualN ? nb / 2 : nb;
+      const int64_t tiles = ceil_div(g.m, 128 * cg) * ceil_div(g.n, tn) * (g.dual == kDualM ? 2 : 1);
+      const int64_t slots = sms / cg;
+      const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(kb / 4, slots / std::max<int64_t>(tiles, 1))) : 1;
+      for (int64_t sp = 1; sp <= most; ++sp) {
+        const double t_kb = nb / 256.0 * 0.28;
+        const double t = ceil_div(tiles * sp, slots) * (ceil_div(kb, sp) * t_kb + 1.0) + (sp > 1 ? 4.0 : 0.0);
+        if (t < best) {
+          best = t;
+          g.cg = cg;
+          g.nb = nb;
+          g.splits = (int)sp;
+        }
+      }
+    }
+}
+
+cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
+  if (g.m <= 0 || g.n <= 0 || g.k <= 0) return cudaErrorInvalidValue;
+  if (encoder() == nullptr) return cudaErrorNotSupported;
+  // The encoder is a driver call and needs a current context, which a thread
+  // of autograd's may not have yet: setting the device makes it current.
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return e;
+  const int bk = g.type == kE4M3 ? 128 : 64;
+  const bool gated = g.dual == kDualN;
+  const int tn = gated ? g.nb / 2 : g.nb;
+  Maps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  const int na = g.dual == kDualK || g.dual == kDualM ? 2 : 1, nbm = g.dual == kDualK || gated ? 2 : 1;
+  for (int i = 0; i < 2; ++i) {
+    if (!make_map(&maps.a[i], g.a[i < na ? i : 0], g.type, g.major_a, g.m, g.k, kRowsA))
+      return cudaErrorInvalidValue;
+    if (!make_map(&maps.b[i], g.b[i < nbm ? i : 0], g.type, g.major_b, g.n, g.k, gated ? g.nb / 2 : g.nb / g.cg))
+      return cudaErrorInvalidValue;
+  }
+  Args args;
+  args.m = g.m;
+  args.n = g.n;
+  args.mt = (int)ceil_div(g.m, kRowsA * g.cg);
+  args.nt = (int)ceil_div(g.n, tn);
+  args.kb = (int)ceil_div(g.k, bk);
+  args.dual = g.dual;
+  args.splits = g.splits;
+  args.idesc = make_idesc(g);
+  args.part_stride = g.m * g.n * (gated || g.dual == kDualM ? 2 : 1);
+  args.partial = g.partial;
+  args.ep = g.ep;
+  if (g.type == kE4M3)
+    e = gated ? launch_shape<kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
+              : launch_shape<kMajorK, kMajorK, true, false>(g, maps, args, sms, s);
+  else if (gated)
+    e = launch_shape<kMajorK, kMajorK, false, true>(g, maps, args, sms, s);
+  else if (g.major_a == kMajorK && g.major_b == kMajorK)
+    e = launch_shape<kMajorK, kMajorK, false, false>(g, maps, args, sms, s);
+  else if (g.major_a == kMajorK)
+    e = launch_shape<kMajorK, kMajorMN, false, false>(g, maps, args, sms, s);
+  else if (g.major_b == kMajorMN)
+    e = launch_shape<kMajorMN, kMajorMN, false, false>(g, maps, args, sms, s);
+  else
+    return cudaErrorInvalidValue;
+  if (e != cudaSuccess || g.splits <= 1) return e;
+  const int64_t runs = ceil_div(g.n, 8) * g.m * (g.dual == kDualM ? 2 : 1);
+  const int grid = (int)std::min<int64_t>(ceil_div(runs, 256), (int64_t)sms * 8);
+  if (gated)
+    k_join<true><<<grid, 256, 0, s>>>(args);
+  else
+    k_join<false><<<grid, 256, 0, s>>>(args);
+  return cudaGetLastError();
+}
+
+cudaError_t read_status(int* out4, bool clear, cudaStream_t s) {
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_status);
+  if (e != cudaSuccess) return e;
+  e = cudaMemcpyAsync(out4, p, 4 * sizeof(int), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess && clear && out4 != nullptr) e = cudaMemsetAsync(p, 0, 4 * sizeof(int), s);
+  return e != cudaSuccess ? e : cudaStreamSynchronize(s);
+}
+
+}  // namespace dense
+}  // namespace ngl

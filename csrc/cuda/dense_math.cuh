@@ -1,0 +1,230 @@
+// Arithmetic shared by the dense kernels: activations and their derivatives in
+// fp32, conversions, and the epilogue over a run of consecutive columns.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "dense.h"
+#include "ngl_cuda.cuh"
+
+namespace ngl {
+namespace dense {
+
+// 1 / (1 + exp(-z)) with the fast exponential and divide: a few ulp of fp32,
+// two orders below the rounding of a 16-bit result.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+constexpr float kGeluA = 0.7978845608028654f;  // sqrt(2 / pi)
+constexpr float kGeluC = 0.044715f;
+
+__device__ __forceinline__ float act_value(int act, float z) {
+  switch (act) {
+    case kActRelu: return z < 0.0f ? 0.0f : z;  // a NaN stays one
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    // 0.5 (1 + tanh(u)) is the logistic function of 2 u
+    case kActGeluTanh: return z * logistic(2.0f * kGeluA * (z + kGeluC * z * z * z));
+    case kActSilu: return z * logistic(z);
+    default: return z;
+  }
+}
+
+// Value and derivative together.  Beyond |z| = 30 each derivative is 0 or 1
+// to fp32 and the clamp keeps 0 * inf out; a NaN passes.
+__device__ __forceinline__ void act_both(int act, float z, float& v, float& d) {
+  const float c = z != z ? z : fminf(fmaxf(z, -30.0f), 30.0f);
+  switch (act) {
+    case kActRelu:
+      v = z < 0.0f ? 0.0f : z;
+      d = z != z ? z : (z > 0.0f ? 1.0f : 0.0f);
+      break;
+    case kActGelu: {
+      const float phi = 0.5f * (1.0f + erff(c * 0.70710678118654752f));
+      v = z * phi;
+      d = phi + c * 0.3989422804014327f * __expf(-0.5f * c * c);
+      break;
+    }
+    case kActGeluTanh: {
+      const float s = logistic(2.0f * kGeluA * (c + kGeluC * c * c * c));
+      v = z * s;
+      d = s + c * s * (1.0f - s) * (2.0f * kGeluA) * (1.0f + 3.0f * kGeluC * c * c);
+      break;
+    }
+    case kActSilu: {
+      const float s = logistic(c);
+      v = z * s;
+      d = s + c * s * (1.0f - s);
+      break;
+    }
+    default:
+      v = z;
+      d = 1.0f;
+  }
+}
+
+__device__ __forceinline__ float half_to_float(uint16_t h, int type) {
+  return type == kBF16 ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
+}
+__device__ __forceinline__ uint16_t float_to_half(float v, int type) {
+  return type == kBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi, int type) {
+  uint32_t r;
+  if (type == kBF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void unpack_half2(uint32_t w, int type, float& lo, float& hi) {
+  if (type == kBF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+
+// One element at index i of an array of `type` (kF32, kBF16 or kF16).
+__device__ __forceinline__ float get(const void* p, int64_t i, int type) {
+  return type == kF32 ? static_cast<const float*>(p)[i] : half_to_float(static_cast<const uint16_t*>(p)[i], type);
+}
+__device__ __forceinline__ void put(void* p, int64_t i, float v, int type) {
+  if (type == kF32)
+    static_cast<float*>(p)[i] = v;
+  else
+    static_cast<uint16_t*>(p)[i] = float_to_half(v, type);
+}
+
+// C consecutive elements (C a multiple of 8) from index i, `valid` of them
+// inside; `vec` says that the address is 16-byte aligned.
+template <int C>
+__device__ __forceinline__ void get_run(const void* p, int64_t i, int type, int valid, bool vec, float (&v)[C]) {
+  if (valid >= C && vec) {
+    if (type == kF32) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < C / 4; ++j) {
+        const float4 f = q[j];
+        v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+      }
+    } else {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < C / 8; ++j) {
+        const uint4 u = q[j];
+        unpack_half2(u.x, type, v[8 * j], v[8 * j + 1]);
+        unpack_half2(u.y, type, v[8 * j + 2], v[8 * j + 3]);
+        unpack_half2(u.z, type, v[8 * j + 4], v[8 * j + 5]);
+        unpack_half2(u.w, type, v[8 * j + 6], v[8 * j + 7]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] = j < valid ? get(p, i + j, type) : 0.0f;
+  }
+}
+template <int C>
+__device__ __forceinline__ void put_run(void* p, int64_t i, int type, int valid, bool vec, const float (&v)[C]) {
+  if (valid >= C && vec) {
+    if (type == kF32) {
+      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < C / 4; ++j) q[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    } else {
+      uint4* q = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < C / 8; ++j)
+        q[j] = make_uint4(pack_half2(v[8 * j], v[8 * j + 1], type), pack_half2(v[8 * j + 2], v[8 * j + 3], type),
+                          pack_half2(v[8 * j + 4], v[8 * j + 5], type), pack_half2(v[8 * j + 6], v[8 * j + 7], type));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+      if (j < valid) put(p, i + j, v[j], type);
+  }
+}
+
+// Whether runs that start at multiples of 8 columns are 16-byte aligned in
+// every row of a matrix.
+__host__ __device__ inline bool runs_aligned(const void* p, int64_t ld, int elem) {
+  return (reinterpret_cast<uintptr_t>(p) % 16) == 0 && (ld * elem) % 16 == 0;
+}
+__host__ __device__ inline int type_bytes(int type) { return type == kF32 ? 4 : type == kE4M3 ? 1 : 2; }
+
+// Alignment of an epilogue's matrices, worked out once a thread.
+struct EpiVec {
+  bool out, z, res, bias;
+};
+__device__ __forceinline__ EpiVec epi_vec(const Epilogue& e, int64_t n) {
+  EpiVec v;
+  v.out = runs_aligned(e.out[0], e.ldo, type_bytes(e.out_type)) &&
+          runs_aligned(e.out[1], e.ldo, type_bytes(e.out_type));
+  v.z = runs_aligned(e.z[0], n, 2) && runs_aligned(e.z[1], n, 2);
+  v.res = runs_aligned(e.residual, e.ldr, type_bytes(e.out_type));
+  v.bias = runs_aligned(e.bias, 0, 2);
+  return v;
+}
+
+// Columns col .. col + C - 1 of one row of problem `which`: scale, bias, keep
+// z, activation, residual, store.
+template <int C>
+__device__ __forceinline__ void epilogue_run(const Epilogue& e, const EpiVec& ev, int which, int64_t row, int64_t col,
+                                             int64_t n, float (&v)[C]) {
+  const int64_t left = n - col;
+  const int valid = left < C ? (int)left : C;
+  if (valid <= 0) return;
+  float t[C];
+  if (e.row_scale != nullptr) {
+    const float rs = e.row_scale[row];
+    get_run<C>(e.col_scale[0], col, kF32, valid, runs_aligned(e.col_scale[0], 0, 4), t);
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] *= rs * t[j];
+  }
+  if (e.bias != nullptr) {
+    get_run<C>(e.bias, col, e.half_type, valid, ev.bias, t);
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] += t[j];
+  }
+  if (e.z[0] != nullptr) put_run<C>(e.z[0], row * n + col, e.half_type, valid, ev.z, v);
+  if (e.act != kActNone) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] = act_value(e.act, v[j]);
+  }
+  if (e.residual != nullptr) {
+    get_run<C>(e.residual, row * e.ldr + col, e.out_type, valid, ev.res, t);
+#pragma unroll
+    for (int j = 0; j < C; ++j) v[j] += t[j];
+  }
+  put_run<C>(e.out[which], row * e.ldo + col, e.out_type, valid, ev.out, v);
+}
+
+// The gated form: g and u are the two projections' columns.
+template <int C>
+__device__ __forceinline__ void epilogue_gated_run(const Epilogue& e, const EpiVec& ev, int64_t row, int64_t col,
+                                                   int64_t n, float (&g)[C], float (&u)[C]) {
+  const int64_t left = n - col;
+  const int valid = left < C ? (int)left : C;
+  if (valid <= 0) return;
+  if (e.row_scale != nullptr) {
+    const float rs = e.row_scale[row];
+    float t[C];
+    get_run<C>(e.col_scale[0], col, kF32, valid, runs_aligned(e.col_scale[0], 0, 4), t);
+#pragma unroll
+    for (int j = 0; j < C; ++j) g[j] *= rs * t[j];
+    get_run<C>(e.col_scale[1], col, kF32, valid, runs_aligned(e.col_scale[1], 0, 4), t);
+#pragma unroll
+    for (int j = 0; j < C; ++j) u[j] *= rs * t[j];
+  }
+  if (e.z[0] != nullptr) {
+    put_run<C>(e.z[0], row * n + col, e.half_type, valid, ev.z, g);
+    put_run<C>(e.z[1], row * n + col, e.half_type, valid, ev.z, u);
+  }
+#pragma unroll
+  for (int j = 0; j < C; ++j) g[j] = act_value(e.act, g[j]) * u[j];
+  put_run<C>(e.out[0], row * e.ldo + col, e.out_type, valid, ev.out, g);
+}
+
+}  // namespace dense
+}  // namespace ngl

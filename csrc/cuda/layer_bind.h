@@ -1,0 +1,66 @@
+// Argument handling shared by the bindings of the dense and norm kernels.
+#pragma once
+#include <torch/extension.h>
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <string>
+
+#include "dense.h"
+
+namespace ngl {
+namespace bind {
+
+using OptTensor = c10::optional<torch::Tensor>;
+
+inline void ck(cudaError_t e, const char* what) { TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e)); }
+
+inline int sm_count(int device) {
+  static int cached[64] = {0};
+  if (device >= 0 && device < 64 && cached[device]) return cached[device];
+  int v = 0;
+  ck(cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, device), "multiprocessor count");
+  if (device >= 0 && device < 64) cached[device] = v;
+  return v;
+}
+
+inline int type_of(torch::ScalarType t) {
+  if (t == torch::kFloat32) return dense::kF32;
+  if (t == torch::kBFloat16) return dense::kBF16;
+  if (t == torch::kHalf) return dense::kF16;
+  if (t == at::kFloat8_e4m3fn) return dense::kE4M3;
+  return -1;
+}
+inline bool is_half(torch::ScalarType t) { return t == torch::kBFloat16 || t == torch::kHalf; }
+
+// Numbers and sizes for messages, as strings: an extension whose C++ library is
+// linked statically cannot stream numbers through torch's message builder.
+inline std::string text(int64_t v) { return std::to_string(v); }
+inline std::string text(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
+}
+
+inline void need_cuda(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor (there is no CPU path)");
+  TORCH_CHECK(t.device() == like.device(), what, " is on cuda:", text(t.get_device()), ", x on cuda:",
+              text(like.get_device()));
+}
+
+// [rows, cols] view of a tensor whose rows lie `ld` elements apart with
+// contiguous columns; a copy where the strides allow no such view.
+struct Rows {
+  torch::Tensor t;  // keeps the memory alive
+  int64_t ld;
+  const void* p() const { return t.data_ptr(); }
+};
+inline Rows rows_of(const torch::Tensor& x, int64_t rows, int64_t cols) {
+  torch::Tensor t = x.dim() == 2 ? x : x.reshape({rows, cols});
+  if ((cols > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < cols)) t = t.contiguous();
+  return {t, rows > 1 ? t.stride(0) : cols};
+}
+
+}  // namespace bind
+}  // namespace ngl
