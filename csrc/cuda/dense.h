@@ -33,13 +33,17 @@ struct Epilogue {
   int out_type;    // of out and residual: half_type or kF32
   void* out[2];    // [m, n] each, row stride ldo; the second for kDualM
   int64_t ldo;
-  void* z[2];      // pre-activations kept for the backward pass (half_type, row stride n)
+  uint16_t* z_hi[2];  // pre-activations kept for the backward pass: the upper 16
+  uint8_t* z_lo[2];   // bits of fp32 and the next 8, row stride ldz = kept_ld(n)
+  int64_t ldz;
   const void* bias;
   const void* residual;
   int64_t ldr;
   const float* row_scale;     // [m], 8-bit operands only
   const float* col_scale[2];  // [n]
 };
+
+inline int64_t kept_ld(int64_t n) { return (n + 15) / 16 * 16; }
 
 struct Operand {
   const void* p;
@@ -61,6 +65,9 @@ struct Gemm {
 // Choose cg, nb and splits of a product for `sms` SMs (g.m, n, k, dual set);
 // may_split allows splits > 1.
 void plan(Gemm& g, int sms, bool may_split);
+// Every following product takes this plan (tests and measurements of one tile
+// shape); cg = 0 returns to plan().
+void force_plan(int cg, int nb, int splits);
 int64_t partial_floats(const Gemm& g);
 
 // Enqueue the product.  Every operand must be fit for TMA: base 16-byte
@@ -70,7 +77,7 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s);
 
 // Few rows (m <= kSkinnyRows): one pass over the weights, any alignment.
 // x [m, k] ldx, w [n, k] ldw (two for the gated form).
-constexpr int kSkinnyRows = 32;
+constexpr int kSkinnyRows = 16;
 struct Skinny {
   int64_t m, n, k;
   int type;
@@ -81,16 +88,18 @@ struct Skinny {
 cudaError_t skinny(const Skinny& g, cudaStream_t s);
 
 // ---- elementwise parts of the backward passes
-// dz = dy * act'(z) in half_type (z null: dz = dy, a cast), db[j] = sum_i dz:
-// partial [parts, n] is scratch for db (null: no db).  dy of dy_type.
+// dz = dy * act'(z) in half_type (act none: dz = dy, a cast; z is not read),
+// db[j] = sum_i dz: partial [parts, n] is scratch for db (null: no db).  dy of
+// dy_type; dz null: only db.
 int colsum_parts(int64_t m, int64_t n, int sms);
-cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const void* z, int act, int half_type, int64_t m,
-                         int64_t n, void* dz, float* partial, int parts, void* db, cudaStream_t s);
+cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_t* z_hi, const uint8_t* z_lo, int act,
+                         int half_type, int64_t m, int64_t n, void* dz, float* partial, int parts, void* db,
+                         cudaStream_t s);
 // out[j] = sum of partial[p, j] over p < parts.
 cudaError_t colsum(const float* partial, int parts, int64_t n, void* out, int type, cudaStream_t s);
-// dg = dh * u * act'(g), du = dh * act(g).
-cudaError_t gated_backward(const void* dh, int64_t ldh, const void* g, const void* u, int act, int half_type,
-                           int64_t m, int64_t n, void* dg, void* du, cudaStream_t s);
+// dg = dh * u * act'(g), du = dh * act(g); z_hi/z_lo[0] hold g, [1] u.
+cudaError_t gated_backward(const void* dh, int64_t ldh, const uint16_t* const z_hi[2], const uint8_t* const z_lo[2],
+                           int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int sms, cudaStream_t s);
 // Rows of `elem`-byte elements copied to a row stride of ldd, the tail zeroed.
 cudaError_t repack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int elem,
                    cudaStream_t s);

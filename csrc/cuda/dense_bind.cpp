@@ -88,6 +88,15 @@ std::vector<int64_t> out_shape(const torch::Tensor& x, int64_t n) {
   return v;
 }
 
+// Kept pre-activations of [m, n]: one buffer, the 16-bit plane first.
+torch::Tensor kept_alloc(const Shape& sh, const torch::Tensor& like) {
+  return torch::empty({sh.m * kept_ld(sh.n) * 3}, like.options().dtype(torch::kUInt8));
+}
+uint16_t* kept_hi(const torch::Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
+uint8_t* kept_lo(const torch::Tensor& t, const Shape& sh) {
+  return static_cast<uint8_t*>(t.data_ptr()) + 2 * sh.m * kept_ld(sh.n);
+}
+
 Epilogue empty_epilogue() {
   Epilogue e;
   std::memset(&e, 0, sizeof(e));
@@ -137,7 +146,7 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   auto y = torch::empty(out_shape(x, sh.n), x.options().dtype(out_t));
   torch::Tensor z;
-  if (keep_z) z = torch::empty({sh.m, sh.n}, x.options().dtype(half));
+  if (keep_z) z = kept_alloc(sh, x);
   if (y.numel() == 0) return {y, z};
 
   std::vector<torch::Tensor> keep;
@@ -148,7 +157,11 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
   ep.out_type = type_of(out_t);
   ep.out[0] = y.data_ptr();
   ep.ldo = sh.n;
-  if (keep_z) ep.z[0] = z.data_ptr();
+  ep.ldz = kept_ld(sh.n);
+  if (keep_z) {
+    ep.z_hi[0] = kept_hi(z);
+    ep.z_lo[0] = kept_lo(z, sh);
+  }
   if (bias.has_value()) {
     keep.push_back(bias->contiguous());
     ep.bias = keep.back().data_ptr();
@@ -209,7 +222,7 @@ std::vector<torch::Tensor> linear_backward(torch::Tensor dy, torch::Tensor x, to
   TORCH_CHECK(dy.sizes().vec() == out_shape(x, sh.n), "gradient must have the output's shape");
   TORCH_CHECK(dy.scalar_type() == x.scalar_type() || dy.scalar_type() == torch::kFloat32,
               "gradient must be ", x.scalar_type(), " or float32; got ", dy.scalar_type());
-  TORCH_CHECK(act == kActNone || z.has_value(), "the activation's gradient needs z");
+  TORCH_CHECK(act == kActNone || (z.has_value() && z->numel() == 3 * sh.m * kept_ld(sh.n)), "the activation's gradient needs z");
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   need_cuda(dy, x, "gradient");
   need_cuda(weight, x, "weight");
@@ -234,8 +247,8 @@ std::vector<torch::Tensor> linear_backward(torch::Tensor dy, torch::Tensor x, to
       db = torch::empty({sh.n}, x.options());
       part = torch::empty({parts, sh.n}, x.options().dtype(torch::kFloat32));
     }
-    ck(act_backward(dzr.p(), type_of(dy.scalar_type()), dzr.ld, act != kActNone ? z->data_ptr() : nullptr, act, half,
-                    sh.m, sh.n, dz.defined() ? dz.data_ptr() : nullptr, need_b ? part.data_ptr<float>() : nullptr,
+    ck(act_backward(dzr.p(), type_of(dy.scalar_type()), dzr.ld, act != kActNone ? kept_hi(*z) : nullptr,
+                    act != kActNone ? kept_lo(*z, sh) : nullptr, act, half, sh.m, sh.n, dz.defined() ? dz.data_ptr() : nullptr, need_b ? part.data_ptr<float>() : nullptr,
                     parts, need_b ? db.data_ptr() : nullptr, s),
        "activation gradient");
     keep.push_back(dzr.t);
@@ -295,8 +308,8 @@ std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, 
   auto h = torch::empty(out_shape(x, sh.n), x.options().dtype(out_t));
   torch::Tensor zg, zu;
   if (keep_zs) {
-    zg = torch::empty({sh.m, sh.n}, x.options().dtype(half));
-    zu = torch::empty({sh.m, sh.n}, x.options().dtype(half));
+    zg = kept_alloc(sh, x);
+    zu = kept_alloc(sh, x);
   }
   if (h.numel() == 0) return {h, zg, zu};
   std::vector<torch::Tensor> keep;
@@ -307,9 +320,12 @@ std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, 
   ep.out_type = type_of(out_t);
   ep.out[0] = h.data_ptr();
   ep.ldo = sh.n;
+  ep.ldz = kept_ld(sh.n);
   if (keep_zs) {
-    ep.z[0] = zg.data_ptr();
-    ep.z[1] = zu.data_ptr();
+    ep.z_hi[0] = kept_hi(zg);
+    ep.z_lo[0] = kept_lo(zg, sh);
+    ep.z_hi[1] = kept_hi(zu);
+    ep.z_lo[1] = kept_lo(zu, sh);
   }
   if (fp8) {
     keep.push_back(x_scale->contiguous());
@@ -371,8 +387,11 @@ std::vector<torch::Tensor> gated_backward_(torch::Tensor dh, torch::Tensor x, to
   std::vector<torch::Tensor> keep;
   const Rows dhr = rows_of(dh, sh.m, sh.n);
   auto dg = torch::empty({sh.m, sh.n}, x.options()), du = torch::empty({sh.m, sh.n}, x.options());
-  ck(gated_backward(dhr.p(), dhr.ld, zg.data_ptr(), zu.data_ptr(), act, type_of(x.scalar_type()), sh.m, sh.n,
-                    dg.data_ptr(), du.data_ptr(), s),
+  TORCH_CHECK(zg.numel() == 3 * sh.m * kept_ld(sh.n) && zu.numel() == 3 * sh.m * kept_ld(sh.n), "the gate's gradient needs g and u");
+  const uint16_t* const hi[2] = {kept_hi(zg), kept_hi(zu)};
+  const uint8_t* const lo[2] = {kept_lo(zg, sh), kept_lo(zu, sh)};
+  ck(gated_backward(dhr.p(), dhr.ld, hi, lo, act, type_of(x.scalar_type()), sh.m, sh.n, dg.data_ptr(), du.data_ptr(),
+                    sm_count(x.get_device()), s),
      "gate gradient");
   const Operand og = tma_operand({dg, sh.n}, sh.m, sh.n, keep, s), ou = tma_operand({du, sh.n}, sh.m, sh.n, keep, s);
   if (need_x) {
@@ -415,6 +434,12 @@ std::vector<int64_t> dense_plan(int64_t m, int64_t n, int64_t k, int64_t dual, b
   return {g.cg, g.nb, g.splits};
 }
 
+void dense_force_plan(int64_t cg, int64_t nb, int64_t splits) {
+  TORCH_CHECK(cg == 0 || ((cg == 1 || cg == 2) && (nb == 128 || nb == 256) && splits >= 1 && splits <= 64),
+              "a plan has 1 or 2 CTAs, 128 or 256 columns, 1 to 64 splits");
+  force_plan((int)cg, (int)nb, (int)splits);
+}
+
 std::vector<int64_t> dense_status(int64_t device, bool clear) {
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   int v[4] = {0, 0, 0, 0};
@@ -430,5 +455,6 @@ void register_dense(pybind11::module& m) {
   m.def("gated_forward", &gated_forward);
   m.def("gated_backward", &gated_backward_);
   m.def("dense_plan", &dense_plan);
+  m.def("dense_force_plan", &dense_force_plan);
   m.def("dense_status", &dense_status);
 }

@@ -21,24 +21,27 @@ constexpr int kLanesY = 8;       // threads along the rows
 // dz = dy act'(z), rounded once to the type that the products read; sums of
 // its columns from the unrounded values.  CTA (bx, by): 256 columns, every
 // gridDim.y-th group of 8 rows.
+template <int kAct>
 __global__ void __launch_bounds__(kLanesX* kLanesY) k_act_backward(const void* dy, int dy_type, int64_t ldy,
-                                                                   const void* z, int act, int half_type, int64_t m,
-                                                                   int64_t n, void* dz, float* partial) {
+                                                                   const uint16_t* z_hi, const uint8_t* z_lo,
+                                                                   int half_type, int64_t m, int64_t n, void* dz,
+                                                                   float* partial) {
   const int64_t col = ((int64_t)blockIdx.x * kLanesX + threadIdx.x) * kColGroup;
   const int valid = (int)max64(0, min64(kColGroup, n - col));
-  const bool vdy = runs_aligned(dy, ldy, type_bytes(dy_type)), vz = runs_aligned(z, n, 2), vo = runs_aligned(dz, n, 2);
+  const bool vdy = runs_aligned(dy, ldy, type_bytes(dy_type)), vo = runs_aligned(dz, n, 2);
+  const int64_t ldz = (n + 15) / 16 * 16;
   float sum[kColGroup] = {};
   if (valid > 0) {
 #pragma unroll 2
     for (int64_t r = (int64_t)blockIdx.y * kLanesY + threadIdx.y; r < m; r += (int64_t)gridDim.y * kLanesY) {
       float d[kColGroup], t[kColGroup];
       get_run<kColGroup>(dy, r * ldy + col, dy_type, valid, vdy, d);
-      if (z != nullptr) {
-        get_run<kColGroup>(z, r * n + col, half_type, valid, vz, t);
+      if (kAct != kActNone) {
+        get_kept8(z_hi, z_lo, r * ldz + col, t);
 #pragma unroll
         for (int j = 0; j < kColGroup; ++j) {
           float v, g;
-          act_both(act, t[j], v, g);
+          act_both<kAct>(t[j], v, g);
           d[j] *= g;
         }
       }
@@ -82,77 +85,109 @@ __global__ void __launch_bounds__(32 * kSumY) k_colsum(const float* partial, int
   }
 }
 
-__global__ void __launch_bounds__(256) k_gated_backward(const void* dh, int64_t ldh, const void* g, const void* u,
-                                                        int act, int half_type, int64_t m, int64_t n, void* dg,
-                                                        void* du) {
-  const int64_t nc = (n + 7) / 8;
-  const bool vh = runs_aligned(dh, ldh, 2),
-             vs = runs_aligned(g, n, 2) && runs_aligned(u, n, 2) && runs_aligned(dg, n, 2) && runs_aligned(du, n, 2);
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < nc * m; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / nc, col = (i - row * nc) * 8;
-    const int valid = (int)min64(8, n - col);
-    float d[8], a[8], b[8];
-    get_run<8>(dh, row * ldh + col, half_type, valid, vh, d);
-    get_run<8>(g, row * n + col, half_type, valid, vs, a);
-    get_run<8>(u, row * n + col, half_type, valid, vs, b);
+template <int kAct>
+__global__ void __launch_bounds__(kLanesX* kLanesY) k_gated_backward(const void* dh, int64_t ldh, const uint16_t* g_hi,
+                                                                     const uint8_t* g_lo, const uint16_t* u_hi,
+                                                                     const uint8_t* u_lo, int half_type, int64_t m,
+                                                                     int64_t n, void* dg, void* du) {
+  const int64_t col = ((int64_t)blockIdx.x * kLanesX + threadIdx.x) * kColGroup;
+  const int valid = (int)max64(0, min64(kColGroup, n - col));
+  if (valid <= 0) return;
+  const bool vh = runs_aligned(dh, ldh, 2), vs = runs_aligned(dg, n, 2) && runs_aligned(du, n, 2);
+  const int64_t ldz = (n + 15) / 16 * 16;
+#pragma unroll 2
+  for (int64_t r = (int64_t)blockIdx.y * kLanesY + threadIdx.y; r < m; r += (int64_t)gridDim.y * kLanesY) {
+    float d[kColGroup], a[kColGroup], b[kColGroup];
+    get_run<kColGroup>(dh, r * ldh + col, half_type, valid, vh, d);
+    get_kept8(g_hi, g_lo, r * ldz + col, a);
+    get_kept8(u_hi, u_lo, r * ldz + col, b);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kColGroup; ++j) {
       float v, s;
-      act_both(act, a[j], v, s);
+      act_both<kAct>(a[j], v, s);
       a[j] = d[j] * b[j] * s;
       b[j] = d[j] * v;
     }
-    put_run<8>(dg, row * n + col, half_type, valid, vs, a);
-    put_run<8>(du, row * n + col, half_type, valid, vs, b);
+    put_run<kColGroup>(dg, r * n + col, half_type, valid, vs, a);
+    put_run<kColGroup>(du, r * n + col, half_type, valid, vs, b);
   }
 }
 
+// CTA (bx, by): 8 elements a thread of the rows by, by + gridDim.y, ...  The
+// sources come here because their rows are not 16-byte aligned, so loads are
+// single elements (adjacent threads share the sectors through L1); stores are
+// 8 elements wide.
 template <typename T>
 __global__ void __launch_bounds__(256) k_repack(const T* src, int64_t lds, T* dst, int64_t ldd, int64_t rows,
                                                 int64_t cols) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * ldd;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / ldd, c = i - r * ldd;
-    dst[i] = c < cols ? src[r * lds + c] : T(0);
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (c >= ldd) return;  // ldd is a multiple of 8
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    alignas(16) T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * lds + c + j] : T(0);
+    if (sizeof(T) == 2)
+      *reinterpret_cast<uint4*>(dst + r * ldd + c) = *reinterpret_cast<const uint4*>(v);
+    else
+      *reinterpret_cast<uint2*>(dst + r * ldd + c) = *reinterpret_cast<const uint2*>(v);
   }
 }
 
-int blocks_for(int64_t items) { return (int)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, 148 * 16)); }
+// Rows of the grid for the 256-column kernels: about 8 CTAs an SM.
+int row_ctas(int64_t m, int64_t n, int sms) {
+  const int64_t bx = (n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup);
+  const int64_t want = (int64_t)sms * 8 / std::max<int64_t>(bx, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 65535), (m + kLanesY - 1) / kLanesY));
+}
+
+#define NGL_BY_ACT(call)              \
+  switch (act) {                      \
+    case kActRelu: call(kActRelu); break;         \
+    case kActGelu: call(kActGelu); break;         \
+    case kActGeluTanh: call(kActGeluTanh); break; \
+    case kActSilu: call(kActSilu); break;         \
+    default: call(kActNone); break;               \
+  }
 
 }  // namespace
 
-int colsum_parts(int64_t m, int64_t n, int sms) {
-  const int64_t bx = (n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup);
-  const int64_t want = (int64_t)sms * 6 / std::max<int64_t>(bx, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (m + kLanesY - 1) / kLanesY));
-}
+int colsum_parts(int64_t m, int64_t n, int sms) { return row_ctas(m, n, sms); }
 
 cudaError_t colsum(const float* partial, int parts, int64_t n, void* out, int type, cudaStream_t s) {
   k_colsum<<<(unsigned)((n + 31) / 32), dim3(32, kSumY), 0, s>>>(partial, parts, n, out, type);
   return cudaGetLastError();
 }
 
-cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const void* z, int act, int half_type, int64_t m,
-                         int64_t n, void* dz, float* partial, int parts, void* db, cudaStream_t s) {
+cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_t* z_hi, const uint8_t* z_lo, int act,
+                         int half_type, int64_t m, int64_t n, void* dz, float* partial, int parts, void* db,
+                         cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)parts);
-  k_act_backward<<<grid, dim3(kLanesX, kLanesY), 0, s>>>(dy, dy_type, ldy, z, act, half_type, m, n, dz,
-                                                         db != nullptr ? partial : nullptr);
+#define NGL_CALL(a)                                                                                          \
+  k_act_backward<a><<<grid, dim3(kLanesX, kLanesY), 0, s>>>(dy, dy_type, ldy, z_hi, z_lo, half_type, m, n, dz, \
+                                                            db != nullptr ? partial : nullptr)
+  NGL_BY_ACT(NGL_CALL)
+#undef NGL_CALL
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess || db == nullptr ? e : colsum(partial, parts, n, db, half_type, s);
 }
 
-cudaError_t gated_backward(const void* dh, int64_t ldh, const void* g, const void* u, int act, int half_type,
-                           int64_t m, int64_t n, void* dg, void* du, cudaStream_t s) {
+cudaError_t gated_backward(const void* dh, int64_t ldh, const uint16_t* const z_hi[2], const uint8_t* const z_lo[2],
+                           int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int sms, cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
-  k_gated_backward<<<blocks_for(m * ((n + 7) / 8)), 256, 0, s>>>(dh, ldh, g, u, act, half_type, m, n, dg, du);
+  const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)row_ctas(m, n, sms));
+#define NGL_CALL(a)                                                                                             \
+  k_gated_backward<a><<<grid, dim3(kLanesX, kLanesY), 0, s>>>(dh, ldh, z_hi[0], z_lo[0], z_hi[1], z_lo[1], half_type, \
+                                                              m, n, dg, du)
+  NGL_BY_ACT(NGL_CALL)
+#undef NGL_CALL
   return cudaGetLastError();
 }
 
 cudaError_t repack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int elem,
                    cudaStream_t s) {
   if (rows <= 0 || cols <= 0) return cudaErrorInvalidValue;
-  const int grid = blocks_for(rows * ldd);
+  const dim3 grid((unsigned)((ldd + 2047) / 2048), (unsigned)std::min<int64_t>(rows, 65535));
   if (elem == 1)
     k_repack<uint8_t><<<grid, 256, 0, s>>>(static_cast<const uint8_t*>(src), lds, static_cast<uint8_t*>(dst), ldd,
                                            rows, cols);

@@ -30,6 +30,7 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kRowsA = 128;       // A rows of one CTA
 constexpr int kBlockBytes = 128;  // bytes of k in one stage
+constexpr int kStageBytes = 4096;  // staging of an epilogue warp
 constexpr uint64_t kWaitNs = 4000000000ull;
 constexpr uint64_t kDrainNs = 100000000ull;
 
@@ -37,8 +38,10 @@ __device__ int g_status[4];
 
 struct alignas(64) Maps {
   CUtensorMap a[2], b[2];
+  CUtensorMap out[2], z_hi[2], z_lo[2];  // boxes of 32 rows and 32 columns
 };
 struct Args {
+  int tma_out;       // out (or the splits' partial sums) is written by TMA
   int64_t m, n;
   int mt, nt;        // tiles of one problem along m and n
   int kb;            // k blocks of one operand pair
@@ -184,10 +187,128 @@ struct Shape {
   static constexpr int kBytesA = kRowsA * kBlockBytes;
   static constexpr int kBytesB = kRowsB * kBlockBytes;
   static constexpr int kStage = kBytesA + kBytesB;
-  static constexpr int kStages = (200 * 1024) / kStage > 8 ? 8 : (200 * 1024) / kStage;
+  static constexpr int kStages = (192 * 1024) / kStage > 8 ? 8 : (192 * 1024) / kStage;
   static constexpr int kCols = 2 * NB;  // tensor memory: two accumulators
-  static constexpr int kSmem = kStages * kStage + 1024 /* alignment */ + 256 /* barriers */;
+  static constexpr int kBarBytes = 1024;  // barriers, then staging (1024-byte aligned for its swizzle)
+  static constexpr int kSmem = kStages * kStage + kBarBytes + kEpiWarps * kStageBytes + 1024 /* alignment */;
+  static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 };
+
+// ---- writing a warp's 32 x 32 pieces
+// Pieces go through 4 KB of shared memory a warp: two slots of 32 rows of 64
+// bytes, or one piece of 32 rows of 128 bytes (fp32).  TMA then writes whole
+// rows of a piece, clipped to the matrix; thread-wise stores from the
+// accumulator's layout (a row a thread) write half sectors and slow the
+// operands' loads: 8192 x 5632 x 2048 took 145 us with them, 121 without any.
+struct Writer {
+  uint32_t smem;  // this warp's staging
+  int slot;       // next 2 KB slot
+  bool whole;     // the last piece used both slots
+};
+__device__ __forceinline__ void writer_wait(const Writer& w, int lane) {
+  if (lane == 0) {
+    if (w.whole)
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    else
+      asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void writer_drain(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+__device__ __forceinline__ void writer_send(const CUtensorMap* map, uint32_t src, int x, int y, int z, int lane) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 32 columns of 16 bits of this lane's row: 64-byte swizzle.
+__device__ __forceinline__ void write_piece16(Writer& w, const CUtensorMap* map, int x, int y, const uint32_t (&p)[16],
+                                              int lane) {
+  writer_wait(w, lane);
+  if (w.whole) w.slot = 0;
+  w.whole = false;
+  const uint32_t base = w.smem + w.slot * 2048;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    sts16(base + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+  writer_send(map, base, x, y, 0, lane);
+  w.slot ^= 1;
+}
+// 32 columns of 8 bits.
+__device__ __forceinline__ void write_piece8(Writer& w, const CUtensorMap* map, int x, int y, const uint32_t (&p)[8],
+                                             int lane) {
+  writer_wait(w, lane);
+  if (w.whole) w.slot = 0;
+  w.whole = false;
+  const uint32_t base = w.smem + w.slot * 2048;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    sts16(base + lane * 32 + c * 16, p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+  writer_send(map, base, x, y, 0, lane);
+  w.slot ^= 1;
+}
+// 32 columns of 32 bits: 128-byte swizzle, both slots.
+__device__ __forceinline__ void write_piece32(Writer& w, const CUtensorMap* map, int x, int y, int z,
+                                              const float (&v)[32], int lane) {
+  writer_drain(lane);
+  w.whole = true;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    sts16(w.smem + lane * 128 + ((c ^ (lane & 7)) << 4), __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
+          __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
+  writer_send(map, w.smem, x, y, z, lane);
+}
+__device__ __forceinline__ void write_half(Writer& w, const CUtensorMap* map, int x, int y, int type,
+                                           const float (&v)[32], int lane) {
+  uint32_t p[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) p[j] = pack_half2(v[2 * j], v[2 * j + 1], type);
+  write_piece16(w, map, x, y, p, lane);
+}
+__device__ __forceinline__ void write_kept(Writer& w, const CUtensorMap* hi, const CUtensorMap* lo, int x, int y,
+                                           const float (&v)[32], int lane) {
+  uint32_t u[32], p[16], q[8];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) u[j] = kept_bits(v[j]);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) p[j] = __byte_perm(u[2 * j], u[2 * j + 1], 0x7632);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    q[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0051), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0051),
+                       0x5410);
+  write_piece16(w, hi, x, y, p, lane);
+  write_piece8(w, lo, x, y, q, lane);
+}
+// A piece of a matrix whose rows TMA cannot address (row stride or base not
+// 16-byte aligned): a row at a time, a column a lane, so that the warp writes
+// adjacent elements together.
+__device__ __forceinline__ void write_plain(Writer& w, void* out, int64_t ld, int type, int64_t row0, int64_t col0,
+                                            int64_t m, int64_t n, const float (&v)[32], int lane) {
+  writer_drain(lane);
+  w.whole = false;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.smem + 4 * (lane * 32 + ((j + lane) & 31))), "f"(v[j]) : "memory");
+  __syncwarp();
+  const int rows = (int)min64(32, m - row0);
+  if (col0 + lane < n)
+    for (int r = 0; r < rows; ++r) {
+      float f;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(w.smem + 4 * (r * 32 + ((lane + r) & 31))) : "memory");
+      put(out, (row0 + r) * ld + col0 + lane, f, type);
+    }
+  __syncwarp();
+}
 
 struct Item {
   int prob;     // kDualM: which product
@@ -366,7 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
     // ---- epilogue
     const int quad = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    const EpiVec ev = epi_vec(g.ep, g.n);
+    const EpiVec ev = epi_vec(g.ep);
+    Writer out = {base + S::kStages * S::kStage + S::kBarBytes + (uint32_t)(warp - 4) * kStageBytes, 0, false};
     int buf = 0;
     uint32_t bph = 0;
     for (int64_t w = first; w < items; w += step) {
@@ -378,43 +500,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
       }
       __syncwarp();
       fence_after();
-      const int64_t row = (int64_t)(it.mt * CG + (int)rank) * kRowsA + quad * 32 + lane;
+      const int64_t row0 = (int64_t)(it.mt * CG + (int)rank) * kRowsA + quad * 32, row = row0 + lane;
       const bool inside = row < g.m;
       const uint32_t acc = lanes + buf * NB;
-      const int64_t col0 = (int64_t)it.nt * kTileN;
-      if (kGated) {
 #pragma unroll 1
-        for (int c = half * (kTileN / 2); c < (half + 1) * (kTileN / 2); c += 32) {
-          float v[32], u[32];
-          tmem_load32(acc + c, v);
-          tmem_load32(acc + kTileN + c, u);
-          tmem_load_wait();
-          if (!inside || col0 + c >= g.n) continue;
-          if (g.splits > 1) {
-            const int valid = (int)min64(32, g.n - col0 - c);
-            const bool vec = g.n % 4 == 0;
-            float* p = g.partial + it.split * g.part_stride;
-            put_run<32>(p, row * g.n + col0 + c, kF32, valid, vec, v);
-            put_run<32>(p + g.m * g.n, row * g.n + col0 + c, kF32, valid, vec && (g.m * g.n) % 4 == 0, u);
+      for (int c = half * (kTileN / 2); c < (half + 1) * (kTileN / 2); c += 32) {
+        const int64_t col = (int64_t)it.nt * kTileN + c;
+        if (row0 >= g.m || col >= g.n) break;  // the same for the whole warp
+        const int valid = inside ? (int)min64(32, g.n - col) : 0;
+        float v[32], u[kGated ? 32 : 1];
+        tmem_load32(acc + c, v);
+        if constexpr (kGated) tmem_load32(acc + kTileN + c, u);
+        tmem_load_wait();
+        if (g.splits > 1) {
+          const int z = (it.split * (kGated || g.dual == kDualM ? 2 : 1)) + it.prob;
+          if (g.tma_out) {
+            write_piece32(out, &maps.out[0], (int)col, (int)row0, z, v, lane);
+            if constexpr (kGated) write_piece32(out, &maps.out[0], (int)col, (int)row0, z + 1, u, lane);
           } else {
-            epilogue_gated_run<32>(g.ep, ev, row, col0 + c, g.n, v, u);
+            write_plain(out, g.partial + z * g.m * g.n, g.n, kF32, row0, col, g.m, g.n, v, lane);
+            if constexpr (kGated)
+              write_plain(out, g.partial + (z + 1) * g.m * g.n, g.n, kF32, row0, col, g.m, g.n, u, lane);
           }
+          continue;
         }
-      } else {
-#pragma unroll 1
-        for (int c = half * (NB / 2); c < (half + 1) * (NB / 2); c += 32) {
-          float v[32];
-          tmem_load32(acc + c, v);
-          tmem_load_wait();
-          if (!inside || col0 + c >= g.n) continue;
-          if (g.splits > 1) {
-            float* p = g.partial + it.split * g.part_stride + it.prob * g.m * g.n;
-            put_run<32>(p, row * g.n + col0 + c, kF32, (int)min64(32, g.n - col0 - c),
-                        g.n % 4 == 0 && (g.m * g.n) % 4 == 0, v);
-          } else {
-            epilogue_run<32>(g.ep, ev, it.prob, row, col0 + c, g.n, v);
-          }
+        epi_sums<32>(g.ep, ev, 0, inside ? row : 0, col, valid, v);
+        if constexpr (kGated) epi_sums<32>(g.ep, ev, 1, inside ? row : 0, col, valid, u);
+        if (g.ep.z_hi[0] != nullptr) {
+          write_kept(out, &maps.z_hi[0], &maps.z_lo[0], (int)col, (int)row0, v, lane);
+          if constexpr (kGated) write_kept(out, &maps.z_hi[1], &maps.z_lo[1], (int)col, (int)row0, u, lane);
         }
+        if constexpr (kGated)
+          epi_gate<32>(g.ep, v, u);
+        else
+          epi_finish<32>(g.ep, ev, inside ? row : 0, col, valid, v);
+        if (!g.tma_out)
+          write_plain(out, g.ep.out[it.prob], g.ep.ldo, g.ep.out_type, row0, col, g.m, g.n, v, lane);
+        else if (g.ep.out_type == kF32)
+          write_piece32(out, &maps.out[it.prob], (int)col, (int)row0, 0, v, lane);
+        else
+          write_half(out, &maps.out[it.prob], (int)col, (int)row0, g.ep.out_type, v, lane);
       }
       fence_before();
       __syncwarp();
@@ -424,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
         bph ^= 1u;
       }
     }
+    writer_drain(lane);  // TMA has read the staging before it is given up
   }
   __syncwarp();
   fence_before();
@@ -438,7 +564,7 @@ template <bool kGated>
 __global__ void __launch_bounds__(256) k_join(Args g) {
   const int64_t nc = (g.n + 7) / 8;
   const int probs = g.dual == kDualM ? 2 : 1;
-  const EpiVec ev = epi_vec(g.ep, g.n);
+  const EpiVec ev = epi_vec(g.ep);
   const bool vec = g.n % 4 == 0 && (g.m * g.n) % 4 == 0;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < nc * g.m * probs;
        i += (int64_t)gridDim.x * blockDim.x) {
@@ -498,6 +624,21 @@ bool make_map(CUtensorMap* map, const Operand& o, int type, int major, int64_t r
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A matrix that pieces of 32 x 32 are written to; `layers` of them in a row.
+bool make_out_map(CUtensorMap* map, void* p, int64_t ld, int64_t m, int64_t n, int64_t layers, int bytes) {
+  const cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)m, (cuuint64_t)layers};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * bytes), (cuuint64_t)(m * ld * bytes)};
+  const cuuint32_t box[3] = {32, 32, 1}, es[3] = {1, 1, 1};
+  const CUtensorMapDataType dt = bytes == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUtensorMapSwizzle sw = bytes == 4   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                             : CU_TENSOR_MAP_SWIZZLE_NONE;
+  return encoder()(map, dt, 3, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Instruction descriptor: fp32 sums, operand types and orders, tile size.
 uint32_t make_idesc(const Gemm& g) {
   const uint32_t t = g.type == kBF16 ? 1u : 0u;  // f16 and e4m3 are both 0 in their kinds
@@ -544,20 +685,43 @@ int64_t partial_floats(const Gemm& g) {
   return g.splits > 1 ? (int64_t)g.splits * g.m * g.n * (g.dual == kDualN || g.dual == kDualM ? 2 : 1) : 0;
 }
 
+namespace {
+int g_force[3] = {0, 0, 0};
+}
+void force_plan(int cg, int nb, int splits) {
+  g_force[0] = cg;
+  g_force[1] = nb;
+  g_force[2] = splits;
+}
+
 void plan(Gemm& g, int sms, bool may_split) {
+  if (g_force[0] != 0) {
+    g.cg = g_force[0];
+    g.nb = g_force[1];
+    g.splits = may_split ? g_force[2] : 1;
+    return;
+  }
+  // Time of a plan = waves of tiles x (k blocks x their time + a tile's fill and
+  // last epilogue) + the join of splits.  Microseconds a k block measured with
+  // 4096 x 4096 x 4096 and 8192 x 5632 x 2048: tiles of 128 columns read twice
+  // the operand bytes a product and take 0.7 to 0.8 of the time of 256 columns,
+  // so they win only where they fill the last wave.
   const int bk = g.type == kE4M3 ? 128 : 64;
   const int64_t kb = ceil_div(g.k, bk) * (g.dual == kDualK ? 2 : 1);
+  const int64_t outs = g.dual == kDualN || g.dual == kDualM ? 2 : 1;
   double best = 1e30;
-  for (int cg = 1; cg <= 2; ++cg)
-    for (int nb = 128; nb <= 256; nb += 128) {
+  for (int cg = 2; cg >= 1; --cg)
+    for (int nb = 256; nb >= 128; nb -= 128) {
+      const double t_kb = nb == 256 ? (cg == 2 ? 0.30 : 0.34) : (cg == 2 ? 0.23 : 0.235);
       const int64_t tn = g.dual == kDualN ? nb / 2 : nb;
       const int64_t tiles = ceil_div(g.m, 128 * cg) * ceil_div(g.n, tn) * (g.dual == kDualM ? 2 : 1);
       const int64_t slots = sms / cg;
-      const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(kb / 4, slots / std::max<int64_t>(tiles, 1))) : 1;
+      const int64_t most = may_split ? std::min<int64_t>(32, std::max<int64_t>(1, kb / 4)) : 1;
       for (int64_t sp = 1; sp <= most; ++sp) {
-        const double t_kb = nb / 256.0 * 0.28;
-        const double t = ceil_div(tiles * sp, slots) * (ceil_div(kb, sp) * t_kb + 1.0) + (sp > 1 ? 4.0 : 0.0);
-        if (t < best) {
+        if (sp > 1 && tiles * sp > 2 * slots) break;
+        const double join = sp > 1 ? 3.0 + (double)(sp + 1) * g.m * g.n * outs * 4 / 5e6 : 0.0;
+        const double t = ceil_div(tiles * sp, slots) * (ceil_div(kb, sp) * t_kb + 1.0) + join;
+        if (t < best * 0.999) {
           best = t;
           g.cg = cg;
           g.nb = nb;
@@ -583,9 +747,9 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   std::memset(&maps, 0, sizeof(maps));
   const int na = g.dual == kDualK || g.dual == kDualM ? 2 : 1, nbm = g.dual == kDualK || gated ? 2 : 1;
   for (int i = 0; i < 2; ++i) {
-    if (!make_map(&maps.a[i], g.a[i < na ? i : 0], g.type, g.major_a, g.m, g.k, kRowsA))
+    if (i < na && !make_map(&maps.a[i], g.a[i], g.type, g.major_a, g.m, g.k, kRowsA))
       return cudaErrorInvalidValue;
-    if (!make_map(&maps.b[i], g.b[i < nbm ? i : 0], g.type, g.major_b, g.n, g.k, gated ? g.nb / 2 : g.nb / g.cg))
+    if (i < nbm && !make_map(&maps.b[i], g.b[i], g.type, g.major_b, g.n, g.k, gated ? g.nb / 2 : g.nb / g.cg))
       return cudaErrorInvalidValue;
   }
   Args args;
@@ -600,6 +764,23 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.part_stride = g.m * g.n * (gated || g.dual == kDualM ? 2 : 1);
   args.partial = g.partial;
   args.ep = g.ep;
+  const int probs = g.dual == kDualM ? 2 : 1;
+  if (g.splits > 1) {
+    // runs_aligned asks for whole 16 bytes a row; the layers of a split are rows apart
+    args.tma_out = runs_aligned(g.partial, g.n, 4);
+    if (args.tma_out &&
+        !make_out_map(&maps.out[0], g.partial, g.n, g.m, g.n, (int64_t)g.splits * (gated ? 2 : probs), 4))
+      return cudaErrorInvalidValue;
+  } else {
+    const int bytes = type_bytes(g.ep.out_type);
+    args.tma_out = runs_aligned(g.ep.out[0], g.ep.ldo, bytes) && runs_aligned(g.ep.out[probs - 1], g.ep.ldo, bytes);
+    for (int i = 0; i < probs && args.tma_out; ++i)
+      if (!make_out_map(&maps.out[i], g.ep.out[i], g.ep.ldo, g.m, g.n, 1, bytes)) return cudaErrorInvalidValue;
+    for (int i = 0; i < (gated ? 2 : 1) && g.ep.z_hi[0] != nullptr; ++i)
+      if (!make_out_map(&maps.z_hi[i], g.ep.z_hi[i], g.ep.ldz, g.m, g.n, 1, 2) ||
+          !make_out_map(&maps.z_lo[i], g.ep.z_lo[i], g.ep.ldz, g.m, g.n, 1, 1))
+        return cudaErrorInvalidValue;
+  }
   if (g.type == kE4M3)
     e = gated ? launch_shape<kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
               : launch_shape<kMajorK, kMajorK, true, false>(g, maps, args, sms, s);

@@ -1,12 +1,13 @@
 // Products of few rows (decoding): bound by one pass over the weights.
 //
 // Mathematics: the epilogue of dense.h over z[i, j] = sum_k x[i, k] w[j, k]
-// for up to 32 rows i.  A warp takes 16 weight rows as the 16-row operand of
-// mma m16n8k16 and groups of 8 rows of x as its 8-column operand; the CTA's
-// 8 warps split k and join their sums in shared memory in warp order.  The
-// sum over k may run in any order as long as both operands agree, so each
-// thread loads 16 contiguous bytes of a row straight into its fragment: no
-// shared memory between the weights and the products.
+// for up to 16 rows i.  The rows of x are the 16-row operand of mma m16n8k16
+// and 8 weight rows its 8-column operand; the CTA's 8 warps split k and join
+// their sums in shared memory in warp order.  The sum over k may run in any
+// order as long as both operands agree, so each thread loads 16 contiguous
+// bytes of a row straight into its fragment: no shared memory between the
+// weights and the products, and every load of a batch is in flight before the
+// first product.
 #include "dense.h"
 
 #include <algorithm>
@@ -21,30 +22,39 @@ namespace {
 using namespace ngl::dev;
 
 constexpr int kWarps = 8;
-constexpr int kWRows = 16;
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool bf16) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, bool bf16) {
   if (bf16)
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
         "%2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
         "%2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of row `row` from byte `at` of its k; zero beyond the row's end.
-template <bool kVec>
-__device__ __forceinline__ uint4 load16(const uint8_t* p, int64_t row_bytes, int64_t at, int64_t k_bytes, bool inside,
-                                        int elem) {
+// 16 bytes of a row from byte `at` of its k; zero beyond the row's end.
+// kOnce: weights, which nothing reads again, do not go through L1.
+template <bool kVec, bool kOnce>
+__device__ __forceinline__ uint4 load16(const uint8_t* row, int64_t at, int64_t k_bytes, bool inside, int elem) {
   if (!inside || at >= k_bytes) return make_uint4(0, 0, 0, 0);
-  const uint8_t* q = p + row_bytes + at;
-  if (kVec) return __ldg(reinterpret_cast<const uint4*>(q));
+  const uint8_t* q = row + at;
+  if (kVec) {
+    uint4 v;
+    if (kOnce)
+      asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                   : "l"(q));
+    else
+      v = __ldg(reinterpret_cast<const uint4*>(q));
+    return v;
+  }
   uint32_t w[4] = {0, 0, 0, 0};
   if (elem == 2) {
 #pragma unroll
@@ -65,81 +75,106 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
   return r;
 }
 
-// MT groups of 8 rows of x; kVec: rows 16-byte aligned and k a multiple of 16 bytes.
-template <int MT, bool kGated, bool kFp8, bool kVec>
+// NT groups of 8 weight rows a CTA (of each projection), U 64-byte blocks of k
+// in flight a warp; kHigh: x has more than 8 rows; kVec: rows 16-byte aligned
+// and k a multiple of 16 bytes.
+template <int NT, int U, bool kHigh, bool kGated, bool kFp8, bool kVec>
 __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ Skinny g) {
   constexpr int NW = kGated ? 2 : 1;
   constexpr int elem = kFp8 ? 1 : 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gq = lane >> 2, t = lane & 3;
-  const int64_t j0 = (int64_t)blockIdx.x * kWRows;
+  const int q = lane >> 2, t = lane & 3;
+  const int64_t j0 = (int64_t)blockIdx.x * (8 * NT);
   const int64_t kbytes = g.k * elem;
   const int64_t nblk = (kbytes + 63) / 64;
   const bool bf16 = g.type == kBF16;
-  const uint8_t* x = static_cast<const uint8_t*>(g.x.p);
-  float acc[NW][MT][4];
+  const uint8_t* x0 = static_cast<const uint8_t*>(g.x.p) + (int64_t)q * g.x.ld * elem;
+  const uint8_t* x1 = x0 + 8 * g.x.ld * elem;
+  const bool in0 = q < g.m, in1 = kHigh && q + 8 < g.m;
+  const uint8_t* wr[NW][NT];
+  bool inw[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t row = j0 + 8 * n + q;
+    inw[n] = row < g.n;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) wr[w][n] = static_cast<const uint8_t*>(g.w[w].p) + row * g.w[w].ld * elem;
+  }
+  float acc[NW][NT][4];
 #pragma unroll
   for (int w = 0; w < NW; ++w)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[w][m][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) acc[w][n][i] = 0.0f;
 
-  const bool in0 = j0 + gq < g.n, in1 = j0 + gq + 8 < g.n;
-#pragma unroll 2
-  for (int64_t b = warp; b < nblk; b += kWarps) {
-    const int64_t at = b * 64 + t * 16;
-    uint4 a[NW][2], xb[MT];
+  for (int64_t b0 = warp; b0 < nblk; b0 += kWarps * U) {
+    uint4 wv[U][NW][NT], xa[U], xb[U];
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const uint8_t* p = static_cast<const uint8_t*>(g.w[w].p);
-      a[w][0] = load16<kVec>(p, (j0 + gq) * g.w[w].ld * elem, at, kbytes, in0, elem);
-      a[w][1] = load16<kVec>(p, (j0 + gq + 8) * g.w[w].ld * elem, at, kbytes, in1, elem);
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (b0 + u * kWarps) * 64 + t * 16;
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) wv[u][w][n] = load16<kVec, true>(wr[w][n], at, kbytes, inw[n], elem);
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-      xb[m] = load16<kVec>(x, (int64_t)(m * 8 + gq) * g.x.ld * elem, at, kbytes, m * 8 + gq < g.m, elem);
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (b0 + u * kWarps) * 64 + t * 16;
+      xa[u] = load16<kVec, false>(x0, at, kbytes, in0, elem);
+      if (kHigh) xb[u] = load16<kVec, false>(x1, at, kbytes, in1, elem);
+    }
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const uint32_t r0[4] = {a[w][0].x, a[w][0].y, a[w][0].z, a[w][0].w};
-      const uint32_t r1[4] = {a[w][1].x, a[w][1].y, a[w][1].z, a[w][1].w};
+    for (int u = 0; u < U; ++u) {
+      const uint32_t p[4] = {xa[u].x, xa[u].y, xa[u].z, xa[u].w};
+      uint32_t r[4] = {0, 0, 0, 0};
+      if (kHigh) {
+        r[0] = xb[u].x;
+        r[1] = xb[u].y;
+        r[2] = xb[u].z;
+        r[3] = xb[u].w;
+      }
 #pragma unroll
       for (int h = 0; h < (kFp8 ? 4 : 2); ++h) {
-        uint32_t f[4];
+        uint32_t a0, a1, a2, a3;
         if (kFp8) {
-          f[0] = e4m3x2_to_half2(r0[h]);
-          f[1] = e4m3x2_to_half2(r1[h]);
-          f[2] = e4m3x2_to_half2(r0[h] >> 16);
-          f[3] = e4m3x2_to_half2(r1[h] >> 16);
+          a0 = e4m3x2_to_half2(p[h]);
+          a2 = e4m3x2_to_half2(p[h] >> 16);
+          a1 = kHigh ? e4m3x2_to_half2(r[h]) : 0u;
+          a3 = kHigh ? e4m3x2_to_half2(r[h] >> 16) : 0u;
         } else {
-          f[0] = r0[2 * h];
-          f[1] = r1[2 * h];
-          f[2] = r0[2 * h + 1];
-          f[3] = r1[2 * h + 1];
+          a0 = p[2 * h];
+          a2 = p[2 * h + 1];
+          a1 = r[2 * h];
+          a3 = r[2 * h + 1];
         }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint32_t xr[4] = {xb[m].x, xb[m].y, xb[m].z, xb[m].w};
-          if (kFp8)
-            mma16816(acc[w][m], f, e4m3x2_to_half2(xr[h]), e4m3x2_to_half2(xr[h] >> 16), false);
-          else
-            mma16816(acc[w][m], f, xr[2 * h], xr[2 * h + 1], bf16);
-        }
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 v = wv[u][w][n];
+            const uint32_t s[4] = {v.x, v.y, v.z, v.w};
+            if (kFp8)
+              mma16816(acc[w][n], a0, a1, a2, a3, e4m3x2_to_half2(s[h]), e4m3x2_to_half2(s[h] >> 16), false);
+            else
+              mma16816(acc[w][n], a0, a1, a2, a3, s[2 * h], s[2 * h + 1], bf16);
+          }
       }
     }
   }
 
-  // acc[.][m][i]: weight row gq + 8 (i / 2), x row m * 8 + 2 t + (i & 1)
-  __shared__ float part[kWarps][NW][MT * 8][kWRows + 1];
+  // acc[.][n][i]: x row q + 8 (i / 2), weight row 8 n + 2 t + (i & 1)
+  constexpr int kX = kHigh ? 16 : 8;
+  __shared__ float part[kWarps][NW][kX][8 * NT + 1];
 #pragma unroll
   for (int w = 0; w < NW; ++w)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[warp][w][m * 8 + 2 * t + (i & 1)][gq + 8 * (i >> 1)] = acc[w][m][i];
+      for (int i = 0; i < (kHigh ? 4 : 2); ++i) part[warp][w][q + 8 * (i >> 1)][8 * n + 2 * t + (i & 1)] = acc[w][n][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < MT * 8 * kWRows; i += kWarps * 32) {
-    const int r = i / kWRows, c = i % kWRows;
+  for (int i = threadIdx.x; i < kX * 8 * NT; i += kWarps * 32) {
+    const int r = i / (8 * NT), c = i % (8 * NT);
     const int64_t row = r, col = j0 + c;
     if (row >= g.m || col >= g.n) continue;
     float s[NW];
@@ -147,7 +182,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
     for (int w = 0; w < NW; ++w) {
       s[w] = 0.0f;
 #pragma unroll
-      for (int q = 0; q < kWarps; ++q) s[w] += part[q][w][r][c];
+      for (int o = 0; o < kWarps; ++o) s[w] += part[o][w][r][c];
     }
     const Epilogue& e = g.ep;
     float z = s[0], u = s[NW - 1];
@@ -156,31 +191,33 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
       if (kGated) u *= e.row_scale[row] * e.col_scale[1][col];
     }
     if (!kGated && e.bias != nullptr) z += get(e.bias, col, e.half_type);
-    if (e.z[0] != nullptr) {
-      put(e.z[0], row * g.n + col, z, e.half_type);
-      if (kGated) put(e.z[1], row * g.n + col, u, e.half_type);
+    if (e.z_hi[0] != nullptr) {
+      put_kept1(e.z_hi[0], e.z_lo[0], row * e.ldz + col, z);
+      if (kGated) put_kept1(e.z_hi[1], e.z_lo[1], row * e.ldz + col, u);
     }
-    float y = act_value(e.act, z);
-    if (kGated) y *= u;
-    if (!kGated && e.residual != nullptr) y += get(e.residual, row * e.ldr + col, e.out_type);
-    put(e.out[0], row * e.ldo + col, y, e.out_type);
+    float y[1] = {z};
+    act_run<1>(e.act, y);
+    if (kGated) y[0] *= u;
+    if (!kGated && e.residual != nullptr) y[0] += get(e.residual, row * e.ldr + col, e.out_type);
+    put(e.out[0], row * e.ldo + col, y[0], e.out_type);
   }
 }
 
-template <int MT, bool kGated, bool kFp8>
-cudaError_t launch_mt(const Skinny& g, bool vec, cudaStream_t s) {
-  const unsigned grid = (unsigned)((g.n + kWRows - 1) / kWRows);
+template <int NT, int U, bool kHigh, bool kGated, bool kFp8>
+cudaError_t launch_nt(const Skinny& g, bool vec, cudaStream_t s) {
+  const unsigned grid = (unsigned)((g.n + 8 * NT - 1) / (8 * NT));
   if (vec)
-    k_skinny<MT, kGated, kFp8, true><<<grid, kWarps * 32, 0, s>>>(g);
+    k_skinny<NT, U, kHigh, kGated, kFp8, true><<<grid, kWarps * 32, 0, s>>>(g);
   else
-    k_skinny<MT, kGated, kFp8, false><<<grid, kWarps * 32, 0, s>>>(g);
+    k_skinny<NT, 2, kHigh, kGated, kFp8, false><<<grid, kWarps * 32, 0, s>>>(g);
   return cudaGetLastError();
 }
+// 8 loads of weights in flight a thread.
 template <bool kGated, bool kFp8>
 cudaError_t launch_skinny(const Skinny& g, bool vec, cudaStream_t s) {
-  if (g.m <= 8) return launch_mt<1, kGated, kFp8>(g, vec, s);
-  if (g.m <= 16) return launch_mt<2, kGated, kFp8>(g, vec, s);
-  return launch_mt<4, kGated, kFp8>(g, vec, s);
+  if (g.m <= 8)
+    return kGated ? launch_nt<1, 4, false, kGated, kFp8>(g, vec, s) : launch_nt<1, 8, false, kGated, kFp8>(g, vec, s);
+  return kGated ? launch_nt<1, 4, true, kGated, kFp8>(g, vec, s) : launch_nt<2, 4, true, kGated, kFp8>(g, vec, s);
 }
 
 }  // namespace

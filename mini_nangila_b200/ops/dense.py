@@ -81,8 +81,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     * ``out_dtype`` may also be float32.
 
     The backward pass gives gradients to x, weight, bias and residual.  It
-    keeps the sums before the activation in x's type, and rounds their gradient
-    to it before the two products.
+    keeps the sums before an activation in 24 bits, and rounds their gradient
+    to x's type before the two products.
     """
     if torch.is_autocast_enabled("cuda"):
         x, weight, bias = _autocast(x, weight, bias)
@@ -105,7 +105,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
 
     Types and 8-bit operands as in ``linear``: ``x_scale`` one float32 a row,
     ``gate_scale`` and ``up_scale`` one an output feature.  The backward pass
-    keeps both projections in x's type and gives gradients to x and both
+    keeps both projections in 24 bits and gives gradients to x and both
     weights.
     """
     if torch.is_autocast_enabled("cuda"):
