@@ -65,8 +65,8 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_act_backward(const void* d
   }
 }
 
-// Column sums of [parts, n]: 32 columns a CTA, 16 threads along the parts, joined in their order.
-constexpr int kSumY = 16;
+// Column sums of [parts, n]: 32 columns a CTA, 32 threads along the parts, joined in their order.
+constexpr int kSumY = 32;
 __global__ void __launch_bounds__(32 * kSumY) k_colsum(const float* partial, int parts, int64_t n, void* out, int type) {
   __shared__ float s[kSumY][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;

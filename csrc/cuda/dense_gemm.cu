@@ -38,10 +38,8 @@ __device__ int g_status[4];
 
 struct alignas(64) Maps {
   CUtensorMap a[2], b[2];
-  CUtensorMap out[2], z_hi[2], z_lo[2];  // boxes of 32 rows and 32 columns
 };
 struct Args {
-  int tma_out;       // out (or the splits' partial sums) is written by TMA
   int64_t m, n;
   int mt, nt;        // tiles of one problem along m and n
   int kb;            // k blocks of one operand pair
@@ -189,125 +187,108 @@ struct Shape {
   static constexpr int kStage = kBytesA + kBytesB;
   static constexpr int kStages = (192 * 1024) / kStage > 8 ? 8 : (192 * 1024) / kStage;
   static constexpr int kCols = 2 * NB;  // tensor memory: two accumulators
-  static constexpr int kBarBytes = 1024;  // barriers, then staging (1024-byte aligned for its swizzle)
+  static constexpr int kBarBytes = 256;
   static constexpr int kSmem = kStages * kStage + kBarBytes + kEpiWarps * kStageBytes + 1024 /* alignment */;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 };
 
 // ---- writing a warp's 32 x 32 pieces
-// Pieces go through 4 KB of shared memory a warp: two slots of 32 rows of 64
-// bytes, or one piece of 32 rows of 128 bytes (fp32).  TMA then writes whole
-// rows of a piece, clipped to the matrix; thread-wise stores from the
-// accumulator's layout (a row a thread) write half sectors and slow the
-// operands' loads: 8192 x 5632 x 2048 took 145 us with them, 121 without any.
-struct Writer {
-  uint32_t smem;  // this warp's staging
-  int slot;       // next 2 KB slot
-  bool whole;     // the last piece used both slots
+// The accumulator's layout gives a lane one row; stored so, every store is half
+// a sector in each of 32 rows, and slows the operands' loads (8192 x 5632 x
+// 2048: 145 us; without any stores 121).  A piece goes through 4 KB of shared
+// memory a warp instead, and each store writes 64 adjacent bytes of 8 rows.
+// (138 us.  TMA stores from the same staging took as long, and need a tensor
+// map for each output on the host.)
+struct Piece {
+  uint32_t smem;
+  int64_t row0, col;
+  int rows;  // rows inside the matrix, 1 to 32
+  int cols;  // columns inside, 1 to 32
+  int lane;
 };
-__device__ __forceinline__ void writer_wait(const Writer& w, int lane) {
-  if (lane == 0) {
-    if (w.whole)
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    else
-      asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-  }
-  __syncwarp();
-}
-__device__ __forceinline__ void writer_drain(int lane) {
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-  __syncwarp();
-}
-__device__ __forceinline__ void writer_send(const CUtensorMap* map, uint32_t src, int x, int y, int z, int lane) {
-  fence_proxy_async_smem();
-  __syncwarp();
-  if (lane == 0) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map),
-                 "r"(x), "r"(y), "r"(z), "r"(src)
-                 : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  }
-}
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// 32 columns of 16 bits of this lane's row: 64-byte swizzle.
-__device__ __forceinline__ void write_piece16(Writer& w, const CUtensorMap* map, int x, int y, const uint32_t (&p)[16],
-                                              int lane) {
-  writer_wait(w, lane);
-  if (w.whole) w.slot = 0;
-  w.whole = false;
-  const uint32_t base = w.smem + w.slot * 2048;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    sts16(base + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
-  writer_send(map, base, x, y, 0, lane);
-  w.slot ^= 1;
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
-// 32 columns of 8 bits.
-__device__ __forceinline__ void write_piece8(Writer& w, const CUtensorMap* map, int x, int y, const uint32_t (&p)[8],
-                                             int lane) {
-  writer_wait(w, lane);
-  if (w.whole) w.slot = 0;
-  w.whole = false;
-  const uint32_t base = w.smem + w.slot * 2048;
+// Rows of R 16-byte units (R = 2, 4 or 8): this lane's row from p, then lanes
+// side by side along the rows of `out`, whose rows are 16-byte aligned.  The
+// units of a row are permuted so that both passes are free of bank conflicts.
+template <int R>
+__device__ __forceinline__ void write_units(const Piece& w, void* out, int64_t ld_bytes, int unit_cols,
+                                            const uint32_t (&p)[4 * R]) {
+  auto at = [&](int row, int unit) {
+    const int swap = R == 8 ? row & 7 : R == 4 ? (row >> 1) & 3 : (row >> 2) & 1;
+    return w.smem + (uint32_t)(row * R + (unit ^ swap)) * 16u;
+  };
+  __syncwarp();  // the last piece has been read
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-    sts16(base + lane * 32 + c * 16, p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
-  writer_send(map, base, x, y, 0, lane);
-  w.slot ^= 1;
-}
-// 32 columns of 32 bits: 128-byte swizzle, both slots.
-__device__ __forceinline__ void write_piece32(Writer& w, const CUtensorMap* map, int x, int y, int z,
-                                              const float (&v)[32], int lane) {
-  writer_drain(lane);
-  w.whole = true;
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-    sts16(w.smem + lane * 128 + ((c ^ (lane & 7)) << 4), __float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]),
-          __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
-  writer_send(map, w.smem, x, y, z, lane);
-}
-__device__ __forceinline__ void write_half(Writer& w, const CUtensorMap* map, int x, int y, int type,
-                                           const float (&v)[32], int lane) {
-  uint32_t p[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) p[j] = pack_half2(v[2 * j], v[2 * j + 1], type);
-  write_piece16(w, map, x, y, p, lane);
-}
-__device__ __forceinline__ void write_kept(Writer& w, const CUtensorMap* hi, const CUtensorMap* lo, int x, int y,
-                                           const float (&v)[32], int lane) {
-  uint32_t u[32], p[16], q[8];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) u[j] = kept_bits(v[j]);
-#pragma unroll
-  for (int j = 0; j < 16; ++j) p[j] = __byte_perm(u[2 * j], u[2 * j + 1], 0x7632);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    q[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0051), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0051),
-                       0x5410);
-  write_piece16(w, hi, x, y, p, lane);
-  write_piece8(w, lo, x, y, q, lane);
-}
-// A piece of a matrix whose rows TMA cannot address (row stride or base not
-// 16-byte aligned): a row at a time, a column a lane, so that the warp writes
-// adjacent elements together.
-__device__ __forceinline__ void write_plain(Writer& w, void* out, int64_t ld, int type, int64_t row0, int64_t col0,
-                                            int64_t m, int64_t n, const float (&v)[32], int lane) {
-  writer_drain(lane);
-  w.whole = false;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.smem + 4 * (lane * 32 + ((j + lane) & 31))), "f"(v[j]) : "memory");
+  for (int c = 0; c < R; ++c) sts16(at(w.lane, c), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
   __syncwarp();
-  const int rows = (int)min64(32, m - row0);
-  if (col0 + lane < n)
-    for (int r = 0; r < rows; ++r) {
-      float f;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(w.smem + 4 * (r * 32 + ((lane + r) & 31))) : "memory");
-      put(out, (row0 + r) * ld + col0 + lane, f, type);
+  constexpr int kRowsAtOnce = 32 / R;
+  const int unit = w.lane % R, r0 = w.lane / R;
+  if (unit * unit_cols >= w.cols) return;
+  uint8_t* q = static_cast<uint8_t*>(out) + (w.row0 + r0) * ld_bytes + (w.col / unit_cols + unit) * 16;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int row = i * kRowsAtOnce + r0;
+    const uint4 v = lds16(at(row, unit));
+    if (row < w.rows) *reinterpret_cast<uint4*>(q + (int64_t)i * kRowsAtOnce * ld_bytes) = v;
+  }
+}
+__device__ __forceinline__ void write_kept(const Piece& w, uint16_t* hi, uint8_t* lo, int64_t ld,
+                                           const float (&v)[32]) {
+  uint32_t p[16], q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t a = kept_bits(v[4 * j]), b = kept_bits(v[4 * j + 1]), c = kept_bits(v[4 * j + 2]),
+                   d = kept_bits(v[4 * j + 3]);
+    p[2 * j] = __byte_perm(a, b, 0x7632);
+    p[2 * j + 1] = __byte_perm(c, d, 0x7632);
+    q[j] = __byte_perm(__byte_perm(a, b, 0x0051), __byte_perm(c, d, 0x0051), 0x5410);
+  }
+  write_units<4>(w, hi, ld * 2, 8, p);
+  write_units<2>(w, lo, ld, 16, q);
+}
+// `aligned`: rows of out start on 16 bytes (then n is a multiple of a unit).
+// Otherwise a row at a time, a column a lane.
+__device__ __forceinline__ void write_piece(const Piece& w, void* out, int64_t ld, int type, bool aligned,
+                                            const float (&v)[32]) {
+  if (aligned && type == kF32) {
+    uint32_t p[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) p[j] = __float_as_uint(v[j]);
+    write_units<8>(w, out, ld * 4, 4, p);
+  } else if (aligned) {
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) p[j] = pack_half2(v[2 * j], v[2 * j + 1], type);
+    write_units<4>(w, out, ld * 2, 8, p);
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.smem + 4 * (w.lane * 32 + ((j + w.lane) & 31))), "f"(v[j])
+                   : "memory");
+    __syncwarp();
+    if (w.lane < w.cols) {
+#pragma unroll 8
+      for (int r = 0; r < w.rows; ++r) {
+        float f;
+        asm volatile("ld.shared.f32 %0, [%1];"
+                     : "=f"(f)
+                     : "r"(w.smem + 4 * (r * 32 + ((w.lane + r) & 31)))
+                     : "memory");
+        put(out, (w.row0 + r) * ld + w.col + w.lane, f, type);
+      }
     }
-  __syncwarp();
+  }
 }
 
 struct Item {
@@ -488,7 +469,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
     const int quad = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     const EpiVec ev = epi_vec(g.ep);
-    Writer out = {base + S::kStages * S::kStage + S::kBarBytes + (uint32_t)(warp - 4) * kStageBytes, 0, false};
+    Piece pc;
+    pc.smem = base + S::kStages * S::kStage + S::kBarBytes + (uint32_t)(warp - 4) * kStageBytes;
+    pc.lane = lane;
+    const bool part_vec = runs_aligned(g.partial, g.n, 4) && (g.m * g.n) % 4 == 0;
     int buf = 0;
     uint32_t bph = 0;
     for (int64_t w = first; w < items; w += step) {
@@ -508,38 +492,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
         const int64_t col = (int64_t)it.nt * kTileN + c;
         if (row0 >= g.m || col >= g.n) break;  // the same for the whole warp
         const int valid = inside ? (int)min64(32, g.n - col) : 0;
+        pc.row0 = row0;
+        pc.col = col;
+        pc.rows = (int)min64(32, g.m - row0);
+        pc.cols = (int)min64(32, g.n - col);
         float v[32], u[kGated ? 32 : 1];
         tmem_load32(acc + c, v);
         if constexpr (kGated) tmem_load32(acc + kTileN + c, u);
         tmem_load_wait();
         if (g.splits > 1) {
-          const int z = (it.split * (kGated || g.dual == kDualM ? 2 : 1)) + it.prob;
-          if (g.tma_out) {
-            write_piece32(out, &maps.out[0], (int)col, (int)row0, z, v, lane);
-            if constexpr (kGated) write_piece32(out, &maps.out[0], (int)col, (int)row0, z + 1, u, lane);
-          } else {
-            write_plain(out, g.partial + z * g.m * g.n, g.n, kF32, row0, col, g.m, g.n, v, lane);
-            if constexpr (kGated)
-              write_plain(out, g.partial + (z + 1) * g.m * g.n, g.n, kF32, row0, col, g.m, g.n, u, lane);
-          }
+          float* p = g.partial + ((int64_t)it.split * (kGated || g.dual == kDualM ? 2 : 1) + it.prob) * g.m * g.n;
+          write_piece(pc, p, g.n, kF32, part_vec, v);
+          if constexpr (kGated) write_piece(pc, p + g.m * g.n, g.n, kF32, part_vec, u);
           continue;
         }
         epi_sums<32>(g.ep, ev, 0, inside ? row : 0, col, valid, v);
         if constexpr (kGated) epi_sums<32>(g.ep, ev, 1, inside ? row : 0, col, valid, u);
         if (g.ep.z_hi[0] != nullptr) {
-          write_kept(out, &maps.z_hi[0], &maps.z_lo[0], (int)col, (int)row0, v, lane);
-          if constexpr (kGated) write_kept(out, &maps.z_hi[1], &maps.z_lo[1], (int)col, (int)row0, u, lane);
+          write_kept(pc, g.ep.z_hi[0], g.ep.z_lo[0], g.ep.ldz, v);
+          if constexpr (kGated) write_kept(pc, g.ep.z_hi[1], g.ep.z_lo[1], g.ep.ldz, u);
         }
         if constexpr (kGated)
           epi_gate<32>(g.ep, v, u);
         else
           epi_finish<32>(g.ep, ev, inside ? row : 0, col, valid, v);
-        if (!g.tma_out)
-          write_plain(out, g.ep.out[it.prob], g.ep.ldo, g.ep.out_type, row0, col, g.m, g.n, v, lane);
-        else if (g.ep.out_type == kF32)
-          write_piece32(out, &maps.out[it.prob], (int)col, (int)row0, 0, v, lane);
-        else
-          write_half(out, &maps.out[it.prob], (int)col, (int)row0, g.ep.out_type, v, lane);
+        write_piece(pc, g.ep.out[it.prob], g.ep.ldo, g.ep.out_type, ev.out, v);
       }
       fence_before();
       __syncwarp();
@@ -549,7 +526,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
         bph ^= 1u;
       }
     }
-    writer_drain(lane);  // TMA has read the staging before it is given up
   }
   __syncwarp();
   fence_before();
@@ -622,21 +598,6 @@ bool make_map(CUtensorMap* map, const Operand& o, int type, int major, int64_t r
   return encode(map, dt, 2, const_cast<void*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// A matrix that pieces of 32 x 32 are written to; `layers` of them in a row.
-bool make_out_map(CUtensorMap* map, void* p, int64_t ld, int64_t m, int64_t n, int64_t layers, int bytes) {
-  const cuuint64_t dims[3] = {(cuuint64_t)n, (cuuint64_t)m, (cuuint64_t)layers};
-  const cuuint64_t strides[2] = {(cuuint64_t)(ld * bytes), (cuuint64_t)(m * ld * bytes)};
-  const cuuint32_t box[3] = {32, 32, 1}, es[3] = {1, 1, 1};
-  const CUtensorMapDataType dt = bytes == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                 : bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
-                                              : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  const CUtensorMapSwizzle sw = bytes == 4   ? CU_TENSOR_MAP_SWIZZLE_128B
-                                : bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                             : CU_TENSOR_MAP_SWIZZLE_NONE;
-  return encoder()(map, dt, 3, p, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Instruction descriptor: fp32 sums, operand types and orders, tile size.
@@ -764,23 +725,6 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.part_stride = g.m * g.n * (gated || g.dual == kDualM ? 2 : 1);
   args.partial = g.partial;
   args.ep = g.ep;
-  const int probs = g.dual == kDualM ? 2 : 1;
-  if (g.splits > 1) {
-    // runs_aligned asks for whole 16 bytes a row; the layers of a split are rows apart
-    args.tma_out = runs_aligned(g.partial, g.n, 4);
-    if (args.tma_out &&
-        !make_out_map(&maps.out[0], g.partial, g.n, g.m, g.n, (int64_t)g.splits * (gated ? 2 : probs), 4))
-      return cudaErrorInvalidValue;
-  } else {
-    const int bytes = type_bytes(g.ep.out_type);
-    args.tma_out = runs_aligned(g.ep.out[0], g.ep.ldo, bytes) && runs_aligned(g.ep.out[probs - 1], g.ep.ldo, bytes);
-    for (int i = 0; i < probs && args.tma_out; ++i)
-      if (!make_out_map(&maps.out[i], g.ep.out[i], g.ep.ldo, g.m, g.n, 1, bytes)) return cudaErrorInvalidValue;
-    for (int i = 0; i < (gated ? 2 : 1) && g.ep.z_hi[0] != nullptr; ++i)
-      if (!make_out_map(&maps.z_hi[i], g.ep.z_hi[i], g.ep.ldz, g.m, g.n, 1, 2) ||
-          !make_out_map(&maps.z_lo[i], g.ep.z_lo[i], g.ep.ldz, g.m, g.n, 1, 1))
-        return cudaErrorInvalidValue;
-  }
   if (g.type == kE4M3)
     e = gated ? launch_shape<kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
               : launch_shape<kMajorK, kMajorK, true, false>(g, maps, args, sms, s);

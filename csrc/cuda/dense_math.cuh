@@ -10,9 +10,15 @@
 namespace ngl {
 namespace dense {
 
-// 1 / (1 + exp(-z)) with the fast exponential and divide: a few ulp of fp32,
-// two orders below the rounding of a 16-bit result.
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// 1 / (1 + exp(-z)) from the hardware's base-2 exponential and reciprocal: a few
+// ulp of fp32, two orders below the rounding of a 16-bit result.  An overflowing
+// exponential gives 0.
+__device__ __forceinline__ float logistic(float z) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
 
 constexpr float kGeluA = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluC = 0.044715f;
@@ -156,13 +162,14 @@ __device__ __forceinline__ void put_run(void* p, int64_t i, int type, int valid,
   }
 }
 
-// Pre-activations kept for the backward pass: the upper 24 bits of fp32
-// (rounded), 16 in one plane and 8 in another.  Kept in 16 bits, their rounding
-// would double the error of the gradients, whose own rounding to 16 bits
-// before the products cannot be avoided; 24 bits cost half as much again in
-// bytes and leave no trace.  Both planes have rows of a multiple of 16
+// Pre-activations kept for the backward pass: the upper 24 bits of fp32, 16 in
+// one plane and 8 in another.  Kept in 16 bits, their rounding would double the
+// error of the gradients, whose own rounding to 16 bits before the products
+// cannot be avoided; 24 bits cost half as much again in bytes and leave an
+// error below 2^-15, without a trace.  The rest is cut off, not rounded, so that
+// no NaN turns into a number.  Both planes have rows of a multiple of 16
 // elements (kept_ld) and 16-byte aligned bases.
-__device__ __forceinline__ uint32_t kept_bits(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v) + 0x80u; }
+__device__ __forceinline__ uint32_t kept_bits(float v) { return __float_as_uint(v); }
 template <int C>
 __device__ __forceinline__ void put_kept(uint16_t* hi, uint8_t* lo, int64_t i, int valid, bool vec,
                                          const float (&v)[C]) {

@@ -39,23 +39,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of a row from byte `at` of its k; zero beyond the row's end.
-// kOnce: weights, which nothing reads again, do not go through L1.
-template <bool kVec, bool kOnce>
-__device__ __forceinline__ uint4 load16(const uint8_t* row, int64_t at, int64_t k_bytes, bool inside, int elem) {
-  if (!inside || at >= k_bytes) return make_uint4(0, 0, 0, 0);
-  const uint8_t* q = row + at;
-  if (kVec) {
-    uint4 v;
-    if (kOnce)
-      asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                   : "l"(q));
-    else
-      v = __ldg(reinterpret_cast<const uint4*>(q));
-    return v;
-  }
+// 16 bytes of a row from byte `at` of its k.  Weights, which nothing reads
+// again, do not go through L1.
+__device__ __forceinline__ uint4 load_once(const uint8_t* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+      : "l"(p));
+  return v;
+}
+// The same from any address, zero beyond the row's end.
+template <int elem>
+__device__ __forceinline__ uint4 load_any(const uint8_t* row, int64_t at, int64_t k_bytes) {
   uint32_t w[4] = {0, 0, 0, 0};
+  const uint8_t* q = row + at;
   if (elem == 2) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -75,9 +72,10 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
   return r;
 }
 
-// NT groups of 8 weight rows a CTA (of each projection), U 64-byte blocks of k
-// in flight a warp; kHigh: x has more than 8 rows; kVec: rows 16-byte aligned
-// and k a multiple of 16 bytes.
+// NT groups of 8 weight rows a CTA (of each projection); a warp takes U
+// consecutive 64-byte blocks of k at a time, all in flight at once.  kHigh: x
+// has more than 8 rows; kVec: rows 16-byte aligned and k a multiple of 16
+// bytes.  Rows beyond the last are read as the last: their sums go nowhere.
 template <int NT, int U, bool kHigh, bool kGated, bool kFp8, bool kVec>
 __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ Skinny g) {
   constexpr int NW = kGated ? 2 : 1;
@@ -86,20 +84,15 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
   const int q = lane >> 2, t = lane & 3;
   const int64_t j0 = (int64_t)blockIdx.x * (8 * NT);
   const int64_t kbytes = g.k * elem;
-  const int64_t nblk = (kbytes + 63) / 64;
   const bool bf16 = g.type == kBF16;
-  const uint8_t* x0 = static_cast<const uint8_t*>(g.x.p) + (int64_t)q * g.x.ld * elem;
-  const uint8_t* x1 = x0 + 8 * g.x.ld * elem;
-  const bool in0 = q < g.m, in1 = kHigh && q + 8 < g.m;
+  const uint8_t* x0 = static_cast<const uint8_t*>(g.x.p) + min64(q, g.m - 1) * g.x.ld * elem;
+  const uint8_t* x1 = static_cast<const uint8_t*>(g.x.p) + min64(q + 8, g.m - 1) * g.x.ld * elem;
   const uint8_t* wr[NW][NT];
-  bool inw[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int64_t row = j0 + 8 * n + q;
-    inw[n] = row < g.n;
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int w = 0; w < NW; ++w) wr[w][n] = static_cast<const uint8_t*>(g.w[w].p) + row * g.w[w].ld * elem;
-  }
+    for (int w = 0; w < NW; ++w)
+      wr[w][n] = static_cast<const uint8_t*>(g.w[w].p) + min64(j0 + 8 * n + q, g.n - 1) * g.w[w].ld * elem;
   float acc[NW][NT][4];
 #pragma unroll
   for (int w = 0; w < NW; ++w)
@@ -108,21 +101,39 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[w][n][i] = 0.0f;
 
-  for (int64_t b0 = warp; b0 < nblk; b0 += kWarps * U) {
+  for (int64_t b0 = (int64_t)warp * (U * 64); b0 < kbytes; b0 += kWarps * U * 64) {
     uint4 wv[U][NW][NT], xa[U], xb[U];
+    if (kVec && b0 + U * 64 <= kbytes) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (b0 + u * kWarps) * 64 + t * 16;
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = b0 + u * 64 + t * 16;
 #pragma unroll
-      for (int w = 0; w < NW; ++w)
+        for (int w = 0; w < NW; ++w)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) wv[u][w][n] = load16<kVec, true>(wr[w][n], at, kbytes, inw[n], elem);
-    }
+          for (int n = 0; n < NT; ++n) wv[u][w][n] = load_once(wr[w][n] + at);
+      }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (b0 + u * kWarps) * 64 + t * 16;
-      xa[u] = load16<kVec, false>(x0, at, kbytes, in0, elem);
-      if (kHigh) xb[u] = load16<kVec, false>(x1, at, kbytes, in1, elem);
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = b0 + u * 64 + t * 16;
+        xa[u] = __ldg(reinterpret_cast<const uint4*>(x0 + at));
+        if (kHigh) xb[u] = __ldg(reinterpret_cast<const uint4*>(x1 + at));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = b0 + u * 64 + t * 16;
+        const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            wv[u][w][n] = kVec ? (at < kbytes ? load_once(wr[w][n] + at) : none) : load_any<elem>(wr[w][n], at, kbytes);
+        xa[u] = kVec ? (at < kbytes ? __ldg(reinterpret_cast<const uint4*>(x0 + at)) : none)
+                     : load_any<elem>(x0, at, kbytes);
+        if (kHigh)
+          xb[u] = kVec ? (at < kbytes ? __ldg(reinterpret_cast<const uint4*>(x1 + at)) : none)
+                       : load_any<elem>(x1, at, kbytes);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {

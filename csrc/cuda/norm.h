@@ -1,6 +1,6 @@
 // Root-mean-square norm of rows with the residual's addition, its backward
 // pass, and the output in e4m3 with one scale a row
-// (csrc/cuda/norm_kernels.cu).
+// (csrc/cuda/norm_forward.cu, norm_backward.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -1,0 +1,155 @@
+// Root-mean-square norm of rows, forward: with the residual's addition, and with
+// an output of the rows' type or of e4m3 with one scale a row (norm.h;
+// norm_common.cuh has the layout).
+#include "norm_common.cuh"
+
+namespace ngl {
+namespace norm {
+namespace {
+
+constexpr float kE4M3Max = 448.0f;
+constexpr float kScaleMin = 1.17549435e-38f;  // 2^-126: a row of zeros keeps a finite inverse
+
+// Four values to e4m3, saturating to +-448; a NaN stays one.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+template <int XT, int ST, int TPR, int VPT, bool kFp8, bool kVec>
+__global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ Forward f) {
+  constexpr int kRows = kCta<TPR> / TPR;
+  __shared__ float sm[kRows][2 * (TPR / 32)];
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, width = (int)f.width;
+  const float inv_width = 1.0f / (float)width;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int turn = 0;
+  float w[VPT][8];
+  Raw<XT> nx[VPT];
+  Raw<ST> nr[VPT];
+  auto run_of = [&](int i, bool inside) {
+    return inside ? max(0, min(8, width - (i * TPR + t) * 8)) : 0;
+  };
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int col = (i * TPR + t) * 8, valid = run_of(i, row < f.rows);
+      nx[i].template load<kVec>(f.x, row * f.ldx + col, valid);
+      if (f.residual != nullptr) nr[i].template load<kVec>(f.residual, row * f.ldr + col, valid);
+    }
+  };
+  int64_t row = (int64_t)blockIdx.x * kRows + group;
+  fetch(row);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) weight_run(f.w, f.w_type, (i * TPR + t) * 8, width, w[i]);
+  // the loop runs the same number of times for all threads of a CTA
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < f.rows; r0 += step, row += step) {
+    const bool inside = row < f.rows;
+    float v[VPT][8];
+    float sum[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      nx[i].to(v[i]);
+      if (f.residual != nullptr) {
+        float r[8];
+        nr[i].to(r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+        if (ST != kF32) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const uint32_t h = pack_half2(v[i][j], v[i][j + 1], ST);
+            unpack_half2(h, ST, v[i][j], v[i][j + 1]);
+          }
+        }
+        Raw<ST>::template store<kVec>(f.stream, row * f.width + (i * TPR + t) * 8, run_of(i, inside), v[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[0] += v[i][j] * v[i][j];
+    }
+    fetch(row + step);
+    if (f.w != nullptr) {
+      row_reduce<TPR, 1, SumOp>(sum, sm[group], turn, group);
+      const float inv = rsqrtf(sum[0] * inv_width + f.eps);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * w[i][j];
+    }
+    float q = 1.0f;
+    if (kFp8) {
+      float top[1] = {0.0f};
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top[0] = fmaxf(top[0], fabsf(v[i][j]));
+      row_reduce<TPR, 1, MaxOp>(top, sm[group], turn, group);
+      const float scale = fmaxf(top[0] * (1.0f / kE4M3Max), kScaleMin);
+      q = 1.0f / scale;
+      if (inside && t == 0) f.scale[row] = scale;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int64_t at = row * f.width + (i * TPR + t) * 8;
+      const int valid = run_of(i, inside);
+      if (kFp8) {
+        const uint32_t lo = e4m3x4(v[i][0] * q, v[i][1] * q, v[i][2] * q, v[i][3] * q);
+        const uint32_t hi = e4m3x4(v[i][4] * q, v[i][5] * q, v[i][6] * q, v[i][7] * q);
+        uint8_t* p = static_cast<uint8_t*>(f.y) + at;
+        if (kVec) {
+          if (valid > 0) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < valid) p[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+        }
+      } else {
+        Raw<XT>::template store<kVec>(f.y, at, valid, v[i]);
+      }
+    }
+  }
+}
+
+template <int XT, int ST, int TPR, int VPT, bool kFp8, bool kVec>
+cudaError_t start(const Forward& f, int sms, cudaStream_t st) {
+  constexpr int kRows = kCta<TPR> / TPR;
+  auto* fn = &k_forward<XT, ST, TPR, VPT, kFp8, kVec>;
+  static int fit = 0;  // CTAs of an SM, the same on every GPU this is built for
+  if (fit == 0) {
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, fn, kCta<TPR>, 0);
+    if (e != cudaSuccess) return e;
+  }
+  const int64_t ctas = (f.rows + kRows - 1) / kRows;
+  fn<<<(unsigned)std::min<int64_t>(ctas, (int64_t)sms * std::max(fit, 1)), kCta<TPR>, 0, st>>>(f);
+  return cudaGetLastError();
+}
+template <int XT, int ST, int TPR, int VPT>
+cudaError_t run_forward(const Forward& f, int sms, cudaStream_t st) {
+  const bool vec = f.width % 8 == 0 && runs_aligned(f.x, f.ldx, type_bytes(XT)) &&
+                   runs_aligned(f.residual, f.ldr, type_bytes(ST)) &&
+                   runs_aligned(f.stream, f.width, type_bytes(ST)) && runs_aligned(f.y, 0, 1);
+  if (f.scale != nullptr)
+    return vec ? start<XT, ST, TPR, VPT, true, true>(f, sms, st) : start<XT, ST, TPR, VPT, true, false>(f, sms, st);
+  return vec ? start<XT, ST, TPR, VPT, false, true>(f, sms, st) : start<XT, ST, TPR, VPT, false, false>(f, sms, st);
+}
+template <int XT, int ST>
+cudaError_t forward_of(const Forward& p, int sms, cudaStream_t st) {
+#define NGL_CALL(T, V) run_forward<XT, ST, T, V>(p, sms, st)
+  NGL_SPLITS(NGL_CALL);
+#undef NGL_CALL
+}
+
+}  // namespace
+
+cudaError_t forward(const Forward& f, int sms, cudaStream_t st) {
+  if (f.rows <= 0 || f.width <= 0 || f.width > kMaxWidth) return cudaErrorInvalidValue;
+  if (f.x_type == kF32) return forward_of<kF32, kF32>(f, sms, st);
+  if (f.x_type == kBF16)
+    return f.stream_type == kF32 ? forward_of<kBF16, kF32>(f, sms, st) : forward_of<kBF16, kBF16>(f, sms, st);
+  return f.stream_type == kF32 ? forward_of<kF16, kF32>(f, sms, st) : forward_of<kF16, kF16>(f, sms, st);
+}
+
+}  // namespace norm
+}  // namespace ngl

@@ -14,7 +14,7 @@ E4M3_MAX = 448.0
 # largest |second derivative| of each activation: what an error of z costs in act'(z)
 CURVE = {"none": 0.0, "relu": 0.0, "gelu": 0.8, "gelu_tanh": 0.82, "silu": 0.5}
 SLOPE = 1.13  # largest |first derivative|
-KEPT = 2.0 ** -16  # pre-activations kept in 24 bits: half a step of 16 significant bits, twice over
+KEPT = 2.0 ** -15  # pre-activations kept in 24 bits: one step of 16 significant bits, cut off
 MATH = 2.0 ** -20  # the fast exponential and divide, relative, with room for their arguments
 
 
