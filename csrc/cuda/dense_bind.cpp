@@ -2,6 +2,7 @@
 // from torch's allocator, launches on the current stream of x's device.
 #include "layer_bind.h"
 
+#include <array>
 #include <vector>
 
 #include "dense.h"
@@ -11,16 +12,6 @@ using namespace ngl::dense;
 using namespace ngl::bind;
 
 constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1024;  // tile coordinates are 32-bit
-
-int act_of(const std::string& a) {
-  if (a == "none") return kActNone;
-  if (a == "relu") return kActRelu;
-  if (a == "gelu") return kActGelu;
-  if (a == "gelu_tanh") return kActGeluTanh;
-  if (a == "silu") return kActSilu;
-  TORCH_CHECK(false, "activation must be one of none, relu, gelu, gelu_tanh, silu; got ", a);
-  return -1;
-}
 
 // An operand that TMA can address: itself, or a copy with padded rows.
 Operand tma_operand(const Rows& r, int64_t rows, int64_t cols, std::vector<torch::Tensor>& keep, cudaStream_t s) {
@@ -47,54 +38,59 @@ void run_gemm(Gemm& g, const torch::Tensor& like, std::vector<torch::Tensor>& ke
 struct Shape {
   int64_t m, k, n;
 };
-// Checks shared by both forms; weights[0] is [n, k].
-Shape check_operands(const torch::Tensor& x, const std::vector<std::pair<torch::Tensor, const char*>>& weights,
-                     const OptTensor& x_scale, const std::vector<std::pair<OptTensor, const char*>>& w_scales) {
+void check_weight(const torch::Tensor& x, const torch::Tensor& w, int64_t k, const char* what) {
+  TORCH_CHECK(w.dim() == 2 && w.size(1) == k, what, " must be [out_features, ", text(k), "]; got ", text(w.sizes()));
+  TORCH_CHECK(w.scalar_type() == x.scalar_type(), what, " must be ", x.scalar_type(), " like x; got ",
+              w.scalar_type());
+}
+void check_scale(const OptTensor& s, bool fp8, int64_t n, const char* what) {
+  TORCH_CHECK(fp8 == s.has_value(), what, fp8 ? " is needed with 8-bit operands" : " needs 8-bit operands");
+  if (fp8)
+    TORCH_CHECK(s->scalar_type() == torch::kFloat32 && s->numel() == n, what,
+                " must be float32 with one value a row (", text(n), "); got ", text(s->sizes()));
+}
+// Checks shared by both forms; w2 undefined for the plain one.
+Shape check_operands(const torch::Tensor& x, const torch::Tensor& w, const char* w_name, const torch::Tensor* w2) {
   TORCH_CHECK(x.dim() >= 1, "x needs at least one dimension");
   const auto t = x.scalar_type();
-  const bool fp8 = t == at::kFloat8_e4m3fn;
-  TORCH_CHECK(fp8 || is_half(t), "x must be bfloat16, float16 or float8_e4m3fn; got ", t);
+  TORCH_CHECK(t == at::kFloat8_e4m3fn || is_half(t), "x must be bfloat16, float16 or float8_e4m3fn; got ", t);
   Shape s;
   s.k = x.size(-1);
   TORCH_CHECK(s.k > 0, "x has no features (its last dimension is 0)");
   s.m = x.numel() / s.k;
-  s.n = 0;
-  for (size_t i = 0; i < weights.size(); ++i) {
-    const auto& w = weights[i].first;
-    TORCH_CHECK(w.dim() == 2 && w.size(1) == s.k, weights[i].second, " must be [out_features, ", text(s.k), "]; got ",
-                text(w.sizes()));
-    TORCH_CHECK(w.scalar_type() == t, weights[i].second, " must be ", t, " like x; got ", w.scalar_type());
-    if (i == 0) s.n = w.size(0);
-    TORCH_CHECK(w.size(0) == s.n, "the two projections must have the same out_features; got ", text(s.n), " and ",
-                text(w.size(0)));
+  check_weight(x, w, s.k, w_name);
+  s.n = w.size(0);
+  if (w2 != nullptr) {
+    check_weight(x, *w2, s.k, "w_up");
+    TORCH_CHECK(w2->size(0) == s.n, "the two projections must have the same out_features; got ", text(s.n), " and ",
+                text(w2->size(0)));
   }
   TORCH_CHECK(s.m <= kMaxDim && s.n <= kMaxDim && s.k <= kMaxDim, "a dimension exceeds ", text(kMaxDim));
-  TORCH_CHECK(fp8 == x_scale.has_value(), fp8 ? "8-bit x needs x_scale" : "x_scale needs an 8-bit x");
-  if (fp8)
-    TORCH_CHECK(x_scale->scalar_type() == torch::kFloat32 && x_scale->numel() == s.m,
-                "x_scale must be float32 with one value a row (", text(s.m), "); got ", text(x_scale->sizes()));
-  for (const auto& ws : w_scales) {
-    TORCH_CHECK(fp8 == ws.first.has_value(), ws.second, fp8 ? " is needed with 8-bit weights" : " needs 8-bit weights");
-    if (fp8)
-      TORCH_CHECK(ws.first->scalar_type() == torch::kFloat32 && ws.first->numel() == s.n, ws.second,
-                  " must be float32 with one value an output feature (", text(s.n), "); got ", text(ws.first->sizes()));
-  }
   return s;
 }
 
-std::vector<int64_t> out_shape(const torch::Tensor& x, int64_t n) {
-  auto v = x.sizes().vec();
+using Sizes = c10::SmallVector<int64_t, 6>;
+Sizes out_shape(const torch::Tensor& x, int64_t n) {
+  Sizes v(x.sizes().begin(), x.sizes().end());
   v.back() = n;
   return v;
 }
+bool has_shape(const torch::Tensor& t, const Sizes& v) { return t.sizes() == at::IntArrayRef(v); }
 
 // Kept pre-activations of [m, n]: one buffer, the 16-bit plane first.
 torch::Tensor kept_alloc(const Shape& sh, const torch::Tensor& like) {
-  return torch::empty({sh.m * kept_ld(sh.n) * 3}, like.options().dtype(torch::kUInt8));
+  return new_cuda({sh.m * kept_ld(sh.n) * 3}, torch::kUInt8, like);
 }
 uint16_t* kept_hi(const torch::Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
 uint8_t* kept_lo(const torch::Tensor& t, const Shape& sh) {
   return static_cast<uint8_t*>(t.data_ptr()) + 2 * sh.m * kept_ld(sh.n);
+}
+
+// The elements of t side by side.
+const void* flat(const torch::Tensor& t, std::vector<torch::Tensor>& keep) {
+  if (t.is_contiguous()) return t.data_ptr();
+  keep.push_back(t.contiguous());
+  return keep.back().data_ptr();
 }
 
 Epilogue empty_epilogue() {
@@ -103,25 +99,31 @@ Epilogue empty_epilogue() {
   return e;
 }
 
-// y, z (z undefined unless keep_z).
-std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight, OptTensor bias, OptTensor residual,
-                                          const std::string& activation, OptTensor x_scale, OptTensor w_scale,
-                                          c10::optional<at::ScalarType> out_dtype, bool keep_z) {
-  const int act = act_of(activation);
-  const Shape sh = check_operands(x, {{weight, "weight"}}, x_scale, {{w_scale, "w_scale"}});
+// y, and the kept pre-activations in *kept where it is not null.
+torch::Tensor linear_forward(const torch::Tensor& x, const torch::Tensor& weight, const OptTensor& bias,
+                             const OptTensor& residual, int act, const OptTensor& x_scale, const OptTensor& w_scale,
+                             c10::optional<at::ScalarType> out_dtype, torch::Tensor* kept) {
+  const Shape sh = check_operands(x, weight, "weight", nullptr);
   const bool fp8 = x.scalar_type() == at::kFloat8_e4m3fn;
+  check_scale(x_scale, fp8, sh.m, "x_scale");
+  check_scale(w_scale, fp8, sh.n, "w_scale");
+  const Sizes shape = out_shape(x, sh.n);
+  // 8-bit operands leave the 16-bit type open: out_dtype's, else the bias's, else the residual's, else bfloat16
   auto half = fp8 ? torch::kBFloat16 : x.scalar_type();
-  if (fp8 && out_dtype.has_value() && is_half(*out_dtype)) half = *out_dtype;
-  if (fp8 && bias.has_value() && is_half(bias->scalar_type()) && !(out_dtype.has_value() && is_half(*out_dtype)))
-    half = bias->scalar_type();
+  if (fp8) {
+    if (out_dtype.has_value() && is_half(*out_dtype))
+      half = *out_dtype;
+    else if (bias.has_value() && is_half(bias->scalar_type()))
+      half = bias->scalar_type();
+    else if (residual.has_value() && is_half(residual->scalar_type()))
+      half = residual->scalar_type();
+  }
   auto out_t = half;
   if (residual.has_value()) {
-    if (fp8 && !out_dtype.has_value() && !bias.has_value() && is_half(residual->scalar_type()))
-      half = residual->scalar_type();
     out_t = residual->scalar_type();
     TORCH_CHECK(out_t == half || out_t == torch::kFloat32, "residual must be ", half, " or float32; got ", out_t);
-    TORCH_CHECK(residual->sizes().vec() == out_shape(x, sh.n), "residual must have the output's shape ",
-                text(out_shape(x, sh.n)), "; got ", text(residual->sizes()));
+    TORCH_CHECK(has_shape(*residual, shape), "residual must have the output's shape ", text(shape), "; got ",
+                text(residual->sizes()));
   }
   if (out_dtype.has_value()) {
     TORCH_CHECK(*out_dtype == half || *out_dtype == torch::kFloat32, "out_dtype must be ", half, " or float32; got ",
@@ -131,7 +133,8 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
     out_t = *out_dtype;
   }
   if (bias.has_value()) {
-    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == sh.n, "bias must be [", text(sh.n), "]; got ", text(bias->sizes()));
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == sh.n, "bias must be [", text(sh.n), "]; got ",
+                text(bias->sizes()));
     TORCH_CHECK(bias->scalar_type() == half, "bias must be ", half, "; got ", bias->scalar_type());
   }
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
@@ -144,10 +147,9 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
   }
   const c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
-  auto y = torch::empty(out_shape(x, sh.n), x.options().dtype(out_t));
-  torch::Tensor z;
-  if (keep_z) z = kept_alloc(sh, x);
-  if (y.numel() == 0) return {y, z};
+  auto y = new_cuda(shape, out_t, x);
+  if (kept != nullptr) *kept = kept_alloc(sh, x);
+  if (y.numel() == 0) return y;
 
   std::vector<torch::Tensor> keep;
   const Rows xr = rows_of(x, sh.m, sh.k), wr = rows_of(weight, sh.n, sh.k);
@@ -158,25 +160,22 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
   ep.out[0] = y.data_ptr();
   ep.ldo = sh.n;
   ep.ldz = kept_ld(sh.n);
-  if (keep_z) {
-    ep.z_hi[0] = kept_hi(z);
-    ep.z_lo[0] = kept_lo(z, sh);
+  if (kept != nullptr) {
+    ep.z_hi[0] = kept_hi(*kept);
+    ep.z_lo[0] = kept_lo(*kept, sh);
   }
   if (bias.has_value()) {
-    keep.push_back(bias->contiguous());
-    ep.bias = keep.back().data_ptr();
+    ep.bias = flat(*bias, keep);
   }
   if (residual.has_value()) {
     const Rows rr = rows_of(*residual, sh.m, sh.n);
-    keep.push_back(rr.t);
+    if (!rr.t.is_same(*residual)) keep.push_back(rr.t);
     ep.residual = rr.p();
     ep.ldr = rr.ld;
   }
   if (fp8) {
-    keep.push_back(x_scale->contiguous());
-    ep.row_scale = keep.back().data_ptr<float>();
-    keep.push_back(w_scale->contiguous());
-    ep.col_scale[0] = keep.back().data_ptr<float>();
+    ep.row_scale = static_cast<const float*>(flat(*x_scale, keep));
+    ep.col_scale[0] = static_cast<const float*>(flat(*w_scale, keep));
   }
   if (sh.m <= kSkinnyRows) {
     Skinny g;
@@ -187,7 +186,7 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
     g.w[0] = {wr.p(), wr.ld};
     g.ep = ep;
     ck(skinny(g, s), "linear");
-    return {y, z};
+    return y;
   }
   Gemm g;
   std::memset(&g, 0, sizeof(g));
@@ -199,7 +198,7 @@ std::vector<torch::Tensor> linear_forward(torch::Tensor x, torch::Tensor weight,
   g.b[0] = tma_operand(wr, sh.n, sh.k, keep, s);
   g.ep = ep;
   run_gemm(g, x, keep, s);
-  return {y, z};
+  return y;
 }
 
 // out [m, n] of like's type = A B^T with the given orders; plain epilogue.
@@ -214,15 +213,15 @@ void plain_product(Gemm& g, std::vector<torch::Tensor> outs, const torch::Tensor
 }
 
 // dx, dw, db (undefined where not needed).
-std::vector<torch::Tensor> linear_backward(torch::Tensor dy, torch::Tensor x, torch::Tensor weight, OptTensor z,
-                                           const std::string& activation, bool need_x, bool need_w, bool need_b) {
-  const int act = act_of(activation);
-  const Shape sh = check_operands(x, {{weight, "weight"}}, c10::nullopt, {});
+std::array<torch::Tensor, 3> linear_backward(const torch::Tensor& dy, const torch::Tensor& x,
+                                             const torch::Tensor& weight, const torch::Tensor& z, int act, bool need_x,
+                                             bool need_w, bool need_b) {
+  const Shape sh = check_operands(x, weight, "weight", nullptr);
   TORCH_CHECK(is_half(x.scalar_type()), "no gradient through 8-bit operands");
-  TORCH_CHECK(dy.sizes().vec() == out_shape(x, sh.n), "gradient must have the output's shape");
+  TORCH_CHECK(has_shape(dy, out_shape(x, sh.n)), "gradient must have the output's shape");
   TORCH_CHECK(dy.scalar_type() == x.scalar_type() || dy.scalar_type() == torch::kFloat32,
               "gradient must be ", x.scalar_type(), " or float32; got ", dy.scalar_type());
-  TORCH_CHECK(act == kActNone || (z.has_value() && z->numel() == 3 * sh.m * kept_ld(sh.n)), "the activation's gradient needs z");
+  TORCH_CHECK(act == kActNone || (z.defined() && z.numel() == 3 * sh.m * kept_ld(sh.n)), "the activation's gradient needs z");
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   need_cuda(dy, x, "gradient");
   need_cuda(weight, x, "weight");
@@ -247,8 +246,8 @@ std::vector<torch::Tensor> linear_backward(torch::Tensor dy, torch::Tensor x, to
       db = torch::empty({sh.n}, x.options());
       part = torch::empty({parts, sh.n}, x.options().dtype(torch::kFloat32));
     }
-    ck(act_backward(dzr.p(), type_of(dy.scalar_type()), dzr.ld, act != kActNone ? kept_hi(*z) : nullptr,
-                    act != kActNone ? kept_lo(*z, sh) : nullptr, act, half, sh.m, sh.n, dz.defined() ? dz.data_ptr() : nullptr, need_b ? part.data_ptr<float>() : nullptr,
+    ck(act_backward(dzr.p(), type_of(dy.scalar_type()), dzr.ld, act != kActNone ? kept_hi(z) : nullptr,
+                    act != kActNone ? kept_lo(z, sh) : nullptr, act, half, sh.m, sh.n, dz.defined() ? dz.data_ptr() : nullptr, need_b ? part.data_ptr<float>() : nullptr,
                     parts, need_b ? db.data_ptr() : nullptr, s),
        "activation gradient");
     keep.push_back(dzr.t);
@@ -279,14 +278,15 @@ std::vector<torch::Tensor> linear_backward(torch::Tensor dy, torch::Tensor x, to
   return {dx, dw, db};
 }
 
-// h, g, u (g and u undefined unless keep).
-std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
-                                         const std::string& activation, OptTensor x_scale, OptTensor gate_scale,
-                                         OptTensor up_scale, c10::optional<at::ScalarType> out_dtype, bool keep_zs) {
-  const int act = act_of(activation);
-  const Shape sh = check_operands(x, {{w_gate, "w_gate"}, {w_up, "w_up"}}, x_scale,
-                                  {{gate_scale, "gate_scale"}, {up_scale, "up_scale"}});
+// h, and the kept projections in kept[0] and kept[1] where it is not null.
+torch::Tensor gated_forward(const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Tensor& w_up, int act,
+                            const OptTensor& x_scale, const OptTensor& gate_scale, const OptTensor& up_scale,
+                            c10::optional<at::ScalarType> out_dtype, torch::Tensor* kept) {
+  const Shape sh = check_operands(x, w_gate, "w_gate", &w_up);
   const bool fp8 = x.scalar_type() == at::kFloat8_e4m3fn;
+  check_scale(x_scale, fp8, sh.m, "x_scale");
+  check_scale(gate_scale, fp8, sh.n, "gate_scale");
+  check_scale(up_scale, fp8, sh.n, "up_scale");
   auto half = fp8 ? torch::kBFloat16 : x.scalar_type();
   if (fp8 && out_dtype.has_value() && is_half(*out_dtype)) half = *out_dtype;
   auto out_t = half;
@@ -305,13 +305,12 @@ std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, 
   }
   const c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
-  auto h = torch::empty(out_shape(x, sh.n), x.options().dtype(out_t));
-  torch::Tensor zg, zu;
-  if (keep_zs) {
-    zg = kept_alloc(sh, x);
-    zu = kept_alloc(sh, x);
+  auto h = new_cuda(out_shape(x, sh.n), out_t, x);
+  if (kept != nullptr) {
+    kept[0] = kept_alloc(sh, x);
+    kept[1] = kept_alloc(sh, x);
   }
-  if (h.numel() == 0) return {h, zg, zu};
+  if (h.numel() == 0) return h;
   std::vector<torch::Tensor> keep;
   const Rows xr = rows_of(x, sh.m, sh.k), gr = rows_of(w_gate, sh.n, sh.k), ur = rows_of(w_up, sh.n, sh.k);
   Epilogue ep = empty_epilogue();
@@ -321,19 +320,14 @@ std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, 
   ep.out[0] = h.data_ptr();
   ep.ldo = sh.n;
   ep.ldz = kept_ld(sh.n);
-  if (keep_zs) {
-    ep.z_hi[0] = kept_hi(zg);
-    ep.z_lo[0] = kept_lo(zg, sh);
-    ep.z_hi[1] = kept_hi(zu);
-    ep.z_lo[1] = kept_lo(zu, sh);
+  for (int i = 0; i < 2 && kept != nullptr; ++i) {
+    ep.z_hi[i] = kept_hi(kept[i]);
+    ep.z_lo[i] = kept_lo(kept[i], sh);
   }
   if (fp8) {
-    keep.push_back(x_scale->contiguous());
-    ep.row_scale = keep.back().data_ptr<float>();
-    keep.push_back(gate_scale->contiguous());
-    ep.col_scale[0] = keep.back().data_ptr<float>();
-    keep.push_back(up_scale->contiguous());
-    ep.col_scale[1] = keep.back().data_ptr<float>();
+    ep.row_scale = static_cast<const float*>(flat(*x_scale, keep));
+    ep.col_scale[0] = static_cast<const float*>(flat(*gate_scale, keep));
+    ep.col_scale[1] = static_cast<const float*>(flat(*up_scale, keep));
   }
   if (sh.m <= kSkinnyRows) {
     Skinny g;
@@ -346,7 +340,7 @@ std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, 
     g.w[1] = {ur.p(), ur.ld};
     g.ep = ep;
     ck(skinny(g, s), "gated linear");
-    return {h, zg, zu};
+    return h;
   }
   Gemm g;
   std::memset(&g, 0, sizeof(g));
@@ -359,17 +353,17 @@ std::vector<torch::Tensor> gated_forward(torch::Tensor x, torch::Tensor w_gate, 
   g.b[1] = tma_operand(ur, sh.n, sh.k, keep, s);
   g.ep = ep;
   run_gemm(g, x, keep, s);
-  return {h, zg, zu};
+  return h;
 }
 
 // dx, dw_gate, dw_up (undefined where not needed).
-std::vector<torch::Tensor> gated_backward_(torch::Tensor dh, torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
-                                           torch::Tensor zg, torch::Tensor zu, const std::string& activation,
-                                           bool need_x, bool need_w) {
-  const int act = act_of(activation);
-  const Shape sh = check_operands(x, {{w_gate, "w_gate"}, {w_up, "w_up"}}, c10::nullopt, {});
+std::array<torch::Tensor, 3> gated_gradients(const torch::Tensor& dh, const torch::Tensor& x,
+                                             const torch::Tensor& w_gate, const torch::Tensor& w_up,
+                                             const torch::Tensor& zg, const torch::Tensor& zu, int act, bool need_x,
+                                             bool need_w) {
+  const Shape sh = check_operands(x, w_gate, "w_gate", &w_up);
   TORCH_CHECK(is_half(x.scalar_type()), "no gradient through 8-bit operands");
-  TORCH_CHECK(dh.sizes().vec() == out_shape(x, sh.n), "gradient must have the output's shape");
+  TORCH_CHECK(has_shape(dh, out_shape(x, sh.n)), "gradient must have the output's shape");
   TORCH_CHECK(dh.scalar_type() == x.scalar_type(), "gradient must be ", x.scalar_type(), "; got ", dh.scalar_type());
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   need_cuda(dh, x, "gradient");
@@ -423,6 +417,96 @@ std::vector<torch::Tensor> gated_backward_(torch::Tensor dh, torch::Tensor x, to
   return {dx, dwg, dwu};
 }
 
+// ---- gradients
+namespace ag = torch::autograd;
+
+class LinearFn : public ag::Function<LinearFn> {
+ public:
+  static torch::Tensor forward(ag::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& w,
+                               const OptTensor& bias, const OptTensor& residual, int64_t act) {
+    torch::Tensor kept;
+    auto y = linear_forward(x, w, bias, residual, (int)act, c10::nullopt, c10::nullopt, c10::nullopt,
+                            act != kActNone ? &kept : nullptr);
+    ctx->save_for_backward({x, w, kept});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return y;
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
+    // edges are those of the tensors given, in their order
+    const bool nb = has_b && ctx->needs_input_grad(2), nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+    auto g = linear_backward(grads[0], saved[0], saved[1], saved[2], (int)ctx->saved_data["act"].toInt(),
+                             ctx->needs_input_grad(0), ctx->needs_input_grad(1), nb);
+    return once({g[0], g[1], g[2], nr ? grads[0] : torch::Tensor(), torch::Tensor()}, "linear");
+  }
+};
+
+class GatedFn : public ag::Function<GatedFn> {
+ public:
+  static torch::Tensor forward(ag::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& w_gate,
+                               const torch::Tensor& w_up, int64_t act) {
+    torch::Tensor kept[2];
+    auto h = gated_forward(x, w_gate, w_up, (int)act, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, kept);
+    ctx->save_for_backward({x, w_gate, w_up, kept[0], kept[1]});
+    ctx->saved_data["act"] = act;
+    return h;
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const bool ng = ctx->needs_input_grad(1), nu = ctx->needs_input_grad(2);
+    auto g = gated_gradients(grads[0], s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["act"].toInt(),
+                             ctx->needs_input_grad(0), ng || nu);
+    return once({g[0], ng ? g[1] : torch::Tensor(), nu ? g[2] : torch::Tensor(), torch::Tensor()}, "gated_linear");
+  }
+};
+
+// A tensor in autocast's type, as F.linear would make it (8-bit operands stay).
+torch::Tensor cast(const torch::Tensor& t) {
+  return t.scalar_type() == at::kFloat8_e4m3fn ? t
+                                               : at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), t);
+}
+
+torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int64_t act, OptTensor residual,
+                     OptTensor x_scale, OptTensor w_scale, c10::optional<at::ScalarType> out_dtype) {
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    x = cast(x);
+    weight = cast(weight);
+    if (bias.has_value()) bias = cast(*bias);
+    if (residual.has_value() && residual->scalar_type() != torch::kFloat32 && is_half(x.scalar_type()))
+      residual = residual->to(x.scalar_type());
+  }
+  if (at::GradMode::is_enabled() &&
+      (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual))) {
+    TORCH_CHECK_VALUE(!x_scale.has_value() && !w_scale.has_value() && x.scalar_type() != at::kFloat8_e4m3fn,
+                      "linear: 8-bit operands have no gradient; call it under torch.no_grad()");
+    TORCH_CHECK_VALUE(!out_dtype.has_value() ||
+                          *out_dtype == (residual.has_value() ? residual->scalar_type() : x.scalar_type()),
+                      "linear: out_dtype is fixed by x and residual where gradients are needed");
+    return LinearFn::apply(x, weight, bias, residual, act);
+  }
+  return linear_forward(x, weight, bias, residual, (int)act, x_scale, w_scale, out_dtype, nullptr);
+}
+
+torch::Tensor gated_linear(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, int64_t act, OptTensor x_scale,
+                           OptTensor gate_scale, OptTensor up_scale, c10::optional<at::ScalarType> out_dtype) {
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    x = cast(x);
+    w_gate = cast(w_gate);
+    w_up = cast(w_up);
+  }
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w_gate) || wants_grad(w_up))) {
+    TORCH_CHECK_VALUE(!x_scale.has_value() && x.scalar_type() != at::kFloat8_e4m3fn,
+                      "gated_linear: 8-bit operands have no gradient; call it under torch.no_grad()");
+    TORCH_CHECK_VALUE(!out_dtype.has_value() || *out_dtype == x.scalar_type(),
+                      "gated_linear: out_dtype is x's type where gradients are needed");
+    return GatedFn::apply(x, w_gate, w_up, act);
+  }
+  return gated_forward(x, w_gate, w_up, (int)act, x_scale, gate_scale, up_scale, out_dtype, nullptr);
+}
+
 // (CTAs of a tile, accumulator columns, splits of k) that a product of these
 // sizes takes on `sms` SMs.
 std::vector<int64_t> dense_plan(int64_t m, int64_t n, int64_t k, int64_t dual, bool fp8, int64_t sms) {
@@ -450,10 +534,8 @@ std::vector<int64_t> dense_status(int64_t device, bool clear) {
 }  // namespace
 
 void register_dense(pybind11::module& m) {
-  m.def("linear_forward", &linear_forward);
-  m.def("linear_backward", &linear_backward);
-  m.def("gated_forward", &gated_forward);
-  m.def("gated_backward", &gated_backward_);
+  m.def("linear", &linear);
+  m.def("gated_linear", &gated_linear);
   m.def("dense_plan", &dense_plan);
   m.def("dense_force_plan", &dense_force_plan);
   m.def("dense_status", &dense_status);

@@ -2,8 +2,12 @@
 #pragma once
 #include <torch/extension.h>
 
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <string>
 
@@ -60,6 +64,30 @@ inline Rows rows_of(const torch::Tensor& x, int64_t rows, int64_t cols) {
   torch::Tensor t = x.dim() == 2 ? x : x.reshape({rows, cols});
   if ((cols > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < cols)) t = t.contiguous();
   return {t, rows > 1 ? t.stride(0) : cols};
+}
+
+inline bool wants_grad(const torch::Tensor& t) { return t.requires_grad(); }
+inline bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+
+// New tensors without the dispatcher's cost (a call of few rows is bound by
+// the host).
+inline torch::Tensor new_cuda(at::IntArrayRef sizes, at::ScalarType t, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, t, like.device(), c10::nullopt);
+}
+
+// Gradients have no gradients of their own: one asked for raises.
+inline torch::autograd::variable_list once(torch::autograd::variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::variable_list in;
+  for (auto& g : grads)
+    if (g.defined()) in.push_back(g.detach().set_requires_grad(true));
+  auto fn = std::make_shared<torch::autograd::DelayedError>(
+      std::string("no second derivative of ") + what, (int64_t)in.size());
+  auto out = (*fn)(std::move(in));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
 }
 
 }  // namespace bind

@@ -1,6 +1,7 @@
 // Torch bindings of the norm kernels (norm.h).
 #include "layer_bind.h"
 
+#include <array>
 #include <vector>
 
 #include "norm.h"
@@ -30,19 +31,20 @@ int64_t check_rows(const torch::Tensor& x, const OptTensor& w, const OptTensor& 
   return width;
 }
 
-// y (or codes), scale (undefined unless fp8), stream (undefined without residual).
-std::vector<torch::Tensor> rms_norm_forward(torch::Tensor x, OptTensor weight, double eps, OptTensor residual,
-                                            bool fp8) {
+struct Out {
+  torch::Tensor y, scale, stream;  // scale only in 8 bits, stream only with a residual
+};
+Out run_forward(const torch::Tensor& x, const OptTensor& weight, double eps, const OptTensor& residual, bool fp8) {
   const int64_t width = check_rows(x, weight, residual, eps), rows = x.numel() / width;
   TORCH_CHECK(weight.has_value() || (fp8 && !residual.has_value()), "weight is needed");
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   if (weight.has_value()) need_cuda(*weight, x, "weight");
   if (residual.has_value()) need_cuda(*residual, x, "residual");
   const c10::cuda::CUDAGuard guard(x.device());
-  auto y = torch::empty(x.sizes(), x.options().dtype(fp8 ? at::kFloat8_e4m3fn : x.scalar_type()));
+  auto y = new_cuda(x.sizes(), fp8 ? at::kFloat8_e4m3fn : x.scalar_type(), x);
   torch::Tensor scale, stream;
-  if (fp8) scale = torch::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(torch::kFloat32));
-  if (residual.has_value()) stream = torch::empty(x.sizes(), residual->options());
+  if (fp8) scale = new_cuda(x.sizes().slice(0, x.dim() - 1), torch::kFloat32, x);
+  if (residual.has_value()) stream = new_cuda(x.sizes(), residual->scalar_type(), x);
   if (rows == 0) return {y, scale, stream};
   const Rows xr = rows_of(x, rows, width);
   Rows rr{xr.t, 0};
@@ -71,22 +73,23 @@ std::vector<torch::Tensor> rms_norm_forward(torch::Tensor x, OptTensor weight, d
 }
 
 // dx, dresidual (dx again where the types agree; undefined without residual), dweight.
-std::vector<torch::Tensor> rms_norm_backward(OptTensor dy, OptTensor ds, torch::Tensor s, torch::Tensor weight,
-                                             double eps, at::ScalarType x_type, bool has_residual, bool need_w) {
+std::array<torch::Tensor, 3> gradients(const torch::Tensor& dy, const torch::Tensor& ds, const torch::Tensor& s,
+                                       const torch::Tensor& weight, double eps, at::ScalarType x_type,
+                                       bool has_residual, bool need_w) {
   const int64_t width = s.size(-1), rows = s.numel() / width;
   TORCH_CHECK(s.is_cuda(), "the stream must be a CUDA tensor (there is no CPU path)");
   const c10::cuda::CUDAGuard guard(s.device());
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   const bool split = has_residual && s.scalar_type() != x_type;
-  auto dx = torch::empty(s.sizes(), s.options().dtype(x_type));
+  auto dx = new_cuda(s.sizes(), x_type, s);
   torch::Tensor dres, dw;
-  if (split) dres = torch::empty(s.sizes(), s.options());
-  if (need_w) dw = torch::empty({width}, weight.options());
+  if (split) dres = new_cuda(s.sizes(), s.scalar_type(), s);
+  if (need_w) dw = new_cuda({width}, weight.scalar_type(), s);
   if (rows == 0) {
     if (need_w) dw.zero_();
     return {dx, has_residual ? (split ? dres : dx) : torch::Tensor(), dw};
   }
-  const torch::Tensor dyt = dy.has_value() ? dy->to(x_type) : torch::zeros(s.sizes(), s.options().dtype(x_type));
+  const torch::Tensor dyt = dy.defined() ? dy.to(x_type) : torch::zeros(s.sizes(), s.options().dtype(x_type));
   TORCH_CHECK(dyt.sizes() == s.sizes(), "gradient must have the output's shape");
   const Rows yr = rows_of(dyt, rows, width), sr = rows_of(s, rows, width);
   Rows er{sr.t, 0};
@@ -96,8 +99,8 @@ std::vector<torch::Tensor> rms_norm_backward(OptTensor dy, OptTensor ds, torch::
   b.x_type = type_of(x_type), b.stream_type = type_of(s.scalar_type());
   b.dy = yr.p(), b.lddy = yr.ld;
   b.s = sr.p(), b.lds = sr.ld;
-  if (ds.has_value()) {
-    er = rows_of(ds->to(s.scalar_type()), rows, width);
+  if (ds.defined()) {
+    er = rows_of(ds.to(s.scalar_type()), rows, width);
     b.ds = er.p(), b.ldds = er.ld;
   }
   const auto w = weight.contiguous();
@@ -110,7 +113,7 @@ std::vector<torch::Tensor> rms_norm_backward(OptTensor dy, OptTensor ds, torch::
   b.parts = norm::backward_parts(rows, width, sms);
   torch::Tensor part;
   if (need_w) {
-    part = torch::empty({b.parts, width}, s.options().dtype(torch::kFloat32));
+    part = new_cuda({b.parts, width}, torch::kFloat32, s);
     b.partial = part.data_ptr<float>();
     b.dw = dw.data_ptr();
   }
@@ -118,9 +121,51 @@ std::vector<torch::Tensor> rms_norm_backward(OptTensor dy, OptTensor ds, torch::
   return {dx, has_residual ? (split ? dres : dx) : torch::Tensor(), dw};
 }
 
+namespace ag = torch::autograd;
+
+class NormFn : public ag::Function<NormFn> {
+ public:
+  static ag::variable_list forward(ag::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
+                                   const OptTensor& residual, double eps) {
+    Out o = run_forward(x, weight, eps, residual, false);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({residual.has_value() ? o.stream : x, weight});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    ctx->saved_data["residual"] = residual.has_value();
+    return residual.has_value() ? ag::variable_list{o.y, o.stream} : ag::variable_list{o.y};
+  }
+  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    const bool has_r = ctx->saved_data["residual"].toBool();
+    const torch::Tensor ds = has_r ? grads[1] : torch::Tensor();
+    const torch::Tensor none;
+    if (!grads[0].defined() && !ds.defined()) return {none, none, none, none};
+    const auto saved = ctx->get_saved_variables();
+    const bool nr = has_r && ctx->needs_input_grad(2);
+    auto g = gradients(grads[0], ds, saved[0], saved[1], ctx->saved_data["eps"].toDouble(),
+                       (at::ScalarType)ctx->saved_data["type"].toInt(), has_r, ctx->needs_input_grad(1));
+    return once({ctx->needs_input_grad(0) ? g[0] : none, g[2], nr ? g[1] : none, none}, "rms_norm");
+  }
+};
+
+// (y,) or (y, stream).
+std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, double eps, OptTensor residual) {
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual)))
+    return NormFn::apply(x, weight, residual, eps);
+  Out o = run_forward(x, weight, eps, residual, false);
+  if (residual.has_value()) return {o.y, o.stream};
+  return {o.y};
+}
+std::vector<torch::Tensor> rms_norm_fp8(torch::Tensor x, OptTensor weight, double eps, OptTensor residual) {
+  const at::NoGradGuard no_grad;
+  Out o = run_forward(x, weight, eps, residual, true);
+  if (residual.has_value()) return {o.y, o.scale, o.stream};
+  return {o.y, o.scale};
+}
+
 }  // namespace
 
 void register_norm(pybind11::module& m) {
-  m.def("rms_norm_forward", &rms_norm_forward);
-  m.def("rms_norm_backward", &rms_norm_backward);
+  m.def("rms_norm", &rms_norm);
+  m.def("rms_norm_fp8", &rms_norm_fp8);
 }

@@ -14,56 +14,21 @@ must be built, and tensors must be CUDA tensors: there is no PyTorch fallback.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from .._ext import cuda
 
 ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu")
+_ACT = {a: i for i, a in enumerate(ACTIVATIONS)}
 
 
 class DenseError(RuntimeError):
     """A product gave up waiting for its own copies; its output is incomplete."""
 
 
-def _autocast(*ts):
-    """The tensors in autocast's type (8-bit operands and None stay)."""
-    dt = torch.get_autocast_dtype("cuda")
-    return [t if t is None or t.dtype == torch.float8_e4m3fn or not t.is_floating_point() else t.to(dt) for t in ts]
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        keep_z = activation != "none"
-        y, z = cuda().linear_forward(x, weight, bias, residual, activation, None, None, None, keep_z)
-        ctx.save_for_backward(x, weight, z)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
-        nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx, dw, db = cuda().linear_backward(dy, x, weight, z, ctx.activation, nx, nw, nb)
-        return dx, dw, db, dy if nr else None, None
-
-
-class _Gated(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, activation):
-        h, g, u = cuda().gated_forward(x, w_gate, w_up, activation, None, None, None, None, True)
-        ctx.save_for_backward(x, w_gate, w_up, g, u)
-        ctx.activation = activation
-        return h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh):
-        x, w_gate, w_up, g, u = ctx.saved_tensors
-        nx, ng, nu = ctx.needs_input_grad[:3]
-        dx, dg, du = cuda().gated_backward(dh, x, w_gate, w_up, g, u, ctx.activation, nx, ng or nu)
-        return dx, dg if ng else None, du if nu else None, None
+def _act(activation: str) -> int:
+    try:
+        return _ACT[activation]
+    except KeyError:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}; got {activation!r}") from None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",
@@ -84,18 +49,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     keeps the sums before an activation in 24 bits, and rounds their gradient
     to x's type before the two products.
     """
-    if torch.is_autocast_enabled("cuda"):
-        x, weight, bias = _autocast(x, weight, bias)
-        if residual is not None and residual.dtype != torch.float32 and x.dtype != torch.float8_e4m3fn:
-            residual = residual.to(x.dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        if x_scale is not None or w_scale is not None or x.dtype == torch.float8_e4m3fn:
-            raise ValueError("linear: 8-bit operands have no gradient; call it under torch.no_grad()")
-        if out_dtype is not None and out_dtype != (x.dtype if residual is None else residual.dtype):
-            raise ValueError("linear: out_dtype is fixed by x and residual where gradients are needed")
-        return _Linear.apply(x, weight, bias, residual, activation)
-    return cuda().linear_forward(x, weight, bias, residual, activation, x_scale, w_scale, out_dtype, False)[0]
+    return cuda().linear(x, weight, bias, _act(activation), residual, x_scale, w_scale, out_dtype)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, activation: str = "silu",
@@ -108,15 +62,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     keeps both projections in 24 bits and gives gradients to x and both
     weights.
     """
-    if torch.is_autocast_enabled("cuda"):
-        x, w_gate, w_up = _autocast(x, w_gate, w_up)
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
-        if x_scale is not None or x.dtype == torch.float8_e4m3fn:
-            raise ValueError("gated_linear: 8-bit operands have no gradient; call it under torch.no_grad()")
-        if out_dtype is not None and out_dtype != x.dtype:
-            raise ValueError("gated_linear: out_dtype is x's type where gradients are needed")
-        return _Gated.apply(x, w_gate, w_up, activation)
-    return cuda().gated_forward(x, w_gate, w_up, activation, x_scale, gate_scale, up_scale, out_dtype, False)[0]
+    return cuda().gated_linear(x, w_gate, w_up, _act(activation), x_scale, gate_scale, up_scale, out_dtype)
 
 
 def check(device: int | torch.device | None = None) -> None:

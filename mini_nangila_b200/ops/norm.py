@@ -8,29 +8,8 @@ fallback.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._ext import cuda
-
-
-class _RMSNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, eps, residual):
-        y, _, stream = cuda().rms_norm_forward(x, weight, eps, residual, False)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if residual is None else stream, weight)
-        ctx.eps, ctx.x_type, ctx.has_residual = eps, x.dtype, residual is not None
-        return y if residual is None else (y, stream)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, ds=None):
-        if dy is None and ds is None:
-            return None, None, None, None
-        s, weight = ctx.saved_tensors
-        nx, nw, _, nr = ctx.needs_input_grad
-        dx, dres, dw = cuda().rms_norm_backward(dy, ds, s, weight, ctx.eps, ctx.x_type, ctx.has_residual, nw)
-        return dx if nx else None, dw, None, dres if nr else None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: torch.Tensor | None = None):
@@ -42,11 +21,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
     float32; y has x's type.  Gradients reach x, weight and residual, from
     either output.
     """
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        return _RMSNorm.apply(x, weight, float(eps), residual)
-    y, _, stream = cuda().rms_norm_forward(x, weight, eps, residual, False)
-    return y if residual is None else (y, stream)
+    out = cuda().rms_norm(x, weight, eps, residual)
+    return out[0] if residual is None else tuple(out)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: torch.Tensor | None = None):
@@ -58,13 +34,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, re
     float8_e4m3fn.  A NaN stays one in its place; an infinity makes its row
     NaN.  No gradient.
     """
-    y, scale, stream = cuda().rms_norm_forward(x.detach(), weight.detach(), eps,
-                                               None if residual is None else residual.detach(), True)
-    return (y, scale) if residual is None else (y, scale, stream)
+    return tuple(cuda().rms_norm_fp8(x, weight, eps, residual))
 
 
 def quantize_rows(x: torch.Tensor):
     """``(codes, scale)`` of the rows of x as ``rms_norm_fp8`` makes them: the
     8-bit form of a weight [out_features, in_features] or of activations."""
-    y, scale, _ = cuda().rms_norm_forward(x.detach(), None, 0.0, None, True)
-    return y, scale
+    return tuple(cuda().rms_norm_fp8(x, None, 0.0, None))
