@@ -9,7 +9,7 @@
 //
 // Layout: persistent CTAs, one per SM (or pairs on one tile).  Warp 0 moves
 // 128-byte-wide tiles with TMA, warp 1 issues the products of 128-byte k
-// blocks, warps 4-11 take finished accumulators from tensor memory through
+// blocks, warps 4 on take finished accumulators from tensor memory through
 // the epilogue while the next tile's products run into the other half of
 // tensor memory.
 #include "dense.h"
@@ -26,11 +26,9 @@ namespace {
 
 using namespace ngl::dev;
 
-constexpr int kThreads = 384;
-constexpr int kEpiWarps = 8;
 constexpr int kRowsA = 128;       // A rows of one CTA
 constexpr int kBlockBytes = 128;  // bytes of k in one stage
-constexpr int kStageBytes = 4096;  // staging of an epilogue warp
+constexpr int kStageBytes = 2048;  // staging of an epilogue warp
 constexpr uint64_t kWaitNs = 4000000000ull;
 constexpr uint64_t kDrainNs = 100000000ull;
 
@@ -43,10 +41,11 @@ struct Args {
   int64_t m, n;
   int mt, nt;        // tiles of one problem along m and n
   int kb;            // k blocks of one operand pair
-  int dual, splits;
+  int dual;
+  int64_t whole;     // tiles summed in one piece; those behind them in `splits` pieces
+  int splits;
   uint32_t idesc;
-  int64_t part_stride;  // floats of one split's partial
-  float* partial;
+  float* partial;    // [split tiles, splits, rows of a tile, NB] sums
   Epilogue ep;
 };
 
@@ -179,8 +178,11 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
 template <int kMaj>
 constexpr uint32_t kStep = kMaj == kMajorK ? 32u : 2048u;
 
-template <int CG, int NB>
+// EW: warps of the epilogue.  16 where a tile's products take less time than its
+// epilogue (small k); else 8, whose registers hold everything.
+template <int CG, int NB, int EW>
 struct Shape {
+  static constexpr int kThreads = 128 + 32 * EW;
   static constexpr int kRowsB = NB / CG;  // B rows of one CTA
   static constexpr int kBytesA = kRowsA * kBlockBytes;
   static constexpr int kBytesB = kRowsB * kBlockBytes;
@@ -188,14 +190,14 @@ struct Shape {
   static constexpr int kStages = (192 * 1024) / kStage > 8 ? 8 : (192 * 1024) / kStage;
   static constexpr int kCols = 2 * NB;  // tensor memory: two accumulators
   static constexpr int kBarBytes = 256;
-  static constexpr int kSmem = kStages * kStage + kBarBytes + kEpiWarps * kStageBytes + 1024 /* alignment */;
+  static constexpr int kSmem = kStages * kStage + kBarBytes + EW * kStageBytes + 1024 /* alignment */;
   static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 };
 
 // ---- writing a warp's 32 x 32 pieces
 // The accumulator's layout gives a lane one row; stored so, every store is half
 // a sector in each of 32 rows, and slows the operands' loads (8192 x 5632 x
-// 2048: 145 us; without any stores 121).  A piece goes through 4 KB of shared
+// 2048: 145 us; without any stores 121).  A piece goes through 2 KB of shared
 // memory a warp instead, and each store writes 64 adjacent bytes of 8 rows.
 // (138 us.  TMA stores from the same staging took as long, and need a tensor
 // map for each output on the host.)
@@ -217,14 +219,14 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
                : "memory");
   return v;
 }
-// Rows of R 16-byte units (R = 2, 4 or 8): this lane's row from p, then lanes
+// Rows of R 16-byte units (R = 2 or 4): this lane's row from p, then lanes
 // side by side along the rows of `out`, whose rows are 16-byte aligned.  The
 // units of a row are permuted so that both passes are free of bank conflicts.
 template <int R>
 __device__ __forceinline__ void write_units(const Piece& w, void* out, int64_t ld_bytes, int unit_cols,
-                                            const uint32_t (&p)[4 * R]) {
+                                            const uint32_t (&p)[4 * R], int skip = 0) {
   auto at = [&](int row, int unit) {
-    const int swap = R == 8 ? row & 7 : R == 4 ? (row >> 1) & 3 : (row >> 2) & 1;
+    const int swap = R == 4 ? (row >> 1) & 3 : (row >> 2) & 1;
     return w.smem + (uint32_t)(row * R + (unit ^ swap)) * 16u;
   };
   __syncwarp();  // the last piece has been read
@@ -233,13 +235,44 @@ __device__ __forceinline__ void write_units(const Piece& w, void* out, int64_t l
   __syncwarp();
   constexpr int kRowsAtOnce = 32 / R;
   const int unit = w.lane % R, r0 = w.lane / R;
-  if (unit * unit_cols >= w.cols) return;
-  uint8_t* q = static_cast<uint8_t*>(out) + (w.row0 + r0) * ld_bytes + (w.col / unit_cols + unit) * 16;
+  if (skip + unit * unit_cols >= w.cols) return;
+  uint8_t* q = static_cast<uint8_t*>(out) + (w.row0 + r0) * ld_bytes + ((w.col + skip) / unit_cols + unit) * 16;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int row = i * kRowsAtOnce + r0;
     const uint4 v = lds16(at(row, unit));
     if (row < w.rows) *reinterpret_cast<uint4*>(q + (int64_t)i * kRowsAtOnce * ld_bytes) = v;
+  }
+}
+// A 16-bit piece of the residual: fetched as it is written, a row's units side by
+// side, so that it can be under way before the sums are ready.
+__device__ __forceinline__ void fetch_units(const Piece& w, const void* src, int64_t ld_bytes, uint4 (&r)[4]) {
+  const int unit = w.lane & 3, r0 = w.lane >> 2;
+  const uint8_t* q = static_cast<const uint8_t*>(src) + (w.row0 + r0) * ld_bytes + (w.col / 8 + unit) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = unit * 8 < w.cols && i * 8 + r0 < w.rows
+               ? __ldg(reinterpret_cast<const uint4*>(q + (int64_t)i * 8 * ld_bytes))
+               : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void add_units(const Piece& w, const uint4 (&r)[4], int type, float (&v)[32]) {
+  auto at = [&](int row, int unit) { return w.smem + (uint32_t)(row * 4 + (unit ^ ((row >> 1) & 3))) * 16u; };
+  const int unit = w.lane & 3, r0 = w.lane >> 2;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sts16(at(i * 8 + r0, unit), r[i].x, r[i].y, r[i].z, r[i].w);
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint4 u = lds16(at(w.lane, c));
+    const uint32_t p[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      unpack_half2(p[j], type, lo, hi);
+      v[8 * c + 2 * j] += lo;
+      v[8 * c + 2 * j + 1] += hi;
+    }
   }
 }
 __device__ __forceinline__ void write_kept(const Piece& w, uint16_t* hi, uint8_t* lo, int64_t ld,
@@ -261,31 +294,39 @@ __device__ __forceinline__ void write_kept(const Piece& w, uint16_t* hi, uint8_t
 __device__ __forceinline__ void write_piece(const Piece& w, void* out, int64_t ld, int type, bool aligned,
                                             const float (&v)[32]) {
   if (aligned && type == kF32) {
-    uint32_t p[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) p[j] = __float_as_uint(v[j]);
-    write_units<8>(w, out, ld * 4, 4, p);
+    for (int h = 0; h < 2; ++h) {  // 16 columns at a time
+      uint32_t p[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(v[16 * h + j]);
+      write_units<4>(w, out, ld * 4, 4, p, 16 * h);
+    }
   } else if (aligned) {
     uint32_t p[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) p[j] = pack_half2(v[2 * j], v[2 * j + 1], type);
     write_units<4>(w, out, ld * 2, 8, p);
   } else {
-    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.smem + 4 * (w.lane * 32 + ((j + w.lane) & 31))), "f"(v[j])
-                   : "memory");
-    __syncwarp();
-    if (w.lane < w.cols) {
-#pragma unroll 8
-      for (int r = 0; r < w.rows; ++r) {
-        float f;
-        asm volatile("ld.shared.f32 %0, [%1];"
-                     : "=f"(f)
-                     : "r"(w.smem + 4 * (r * 32 + ((w.lane + r) & 31)))
+    for (int h = 0; h < 2; ++h) {  // 16 columns of 32 rows, two rows a store
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.smem + 4 * (w.lane * 16 + ((j + (w.lane >> 1)) & 15))),
+                     "f"(v[16 * h + j])
                      : "memory");
-        put(out, (w.row0 + r) * ld + w.col + w.lane, f, type);
+      __syncwarp();
+      const int c = w.lane & 15, sub = w.lane >> 4;
+      if (16 * h + c < w.cols) {
+#pragma unroll 8
+        for (int r = sub; r < w.rows; r += 2) {
+          float f;
+          asm volatile("ld.shared.f32 %0, [%1];"
+                       : "=f"(f)
+                       : "r"(w.smem + 4 * (r * 16 + ((c + (r >> 1)) & 15)))
+                       : "memory");
+          put(out, (w.row0 + r) * ld + w.col + 16 * h + c, f, type);
+        }
       }
     }
   }
@@ -294,35 +335,50 @@ __device__ __forceinline__ void write_piece(const Piece& w, void* out, int64_t l
 struct Item {
   int prob;     // kDualM: which product
   int mt, nt;   // tile
-  int split;
   int k0, k1;   // k blocks
+  int64_t part; // slot of `partial`, or -1
 };
-// Work item w.  Groups of 8 rows of tiles sweep the columns together, so that
-// the tiles that run at one time share their operands in L2.
-__device__ __forceinline__ Item item_of(const Args& g, int64_t w) {
+__device__ __forceinline__ int64_t tiles_of(const Args& g) {
+  return (int64_t)g.mt * (g.dual == kDualM ? 2 : 1) * g.nt;
+}
+// Tile t.  Groups of 8 rows of tiles sweep the columns together, so that the
+// tiles that run at one time share their operands in L2.
+__device__ __forceinline__ void tile_of(const Args& g, int64_t t, Item& it) {
   const int rows = g.mt * (g.dual == kDualM ? 2 : 1);
-  const int64_t tiles = (int64_t)rows * g.nt;
-  Item it;
-  it.split = (int)(w / tiles);
-  const int64_t t = w - it.split * tiles;
-  const int per = 8 * g.nt;
-  const int grp = (int)(t / per), in = (int)(t - (int64_t)grp * per);
+  const int64_t per = 8ll * g.nt;
+  const int grp = (int)(t / per), in = (int)(t - grp * per);
   const int h = min(8, rows - grp * 8);
   it.nt = in / h;
   const int r = grp * 8 + in % h;
   it.prob = r / g.mt;
   it.mt = r - it.prob * g.mt;
+}
+// Work item w: a whole tile, or one of the pieces of k of a tile behind them.
+__device__ __forceinline__ Item item_of(const Args& g, int64_t w) {
+  Item it;
   const int kb = g.kb * (g.dual == kDualK ? 2 : 1);
-  it.k0 = (int)((int64_t)kb * it.split / g.splits);
-  it.k1 = (int)((int64_t)kb * (it.split + 1) / g.splits);
+  if (w < g.whole) {
+    tile_of(g, w, it);
+    it.k0 = 0;
+    it.k1 = kb;
+    it.part = -1;
+    return it;
+  }
+  it.part = w - g.whole;
+  const int64_t r = it.part / g.splits;
+  const int sp = (int)(it.part - r * g.splits);
+  tile_of(g, g.whole + r, it);
+  it.k0 = (int)((int64_t)kb * sp / g.splits);
+  it.k1 = (int)((int64_t)kb * (sp + 1) / g.splits);
   return it;
 }
 
-template <int CG, int NB, int MA, int MB, bool kFp8, bool kGated>
-__global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
-  using S = Shape<CG, NB>;
+template <int CG, int NB, int EW, int MA, int MB, bool kFp8, bool kGated>
+__global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant__ Maps maps, const __grid_constant__ Args g) {
+  using S = Shape<CG, NB, EW>;
   constexpr int kBk = kFp8 ? 128 : 64;  // k of one stage
   constexpr int kTileN = kGated ? NB / 2 : NB;
+  constexpr int kGroups = kTileN / 32 < EW / 4 ? kTileN / 32 : EW / 4;  // epilogue warps share a tile's columns
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t bars = base + S::kStages * S::kStage;
@@ -344,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
     }
     for (int b = 0; b < 2; ++b) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(tfull(b)) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tempty(b)), "r"(CG * kEpiWarps) : "memory");
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tempty(b)), "r"(CG * 4 * kGroups) : "memory");
     }
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(drained) : "memory");
     fence_mbar_init();
@@ -355,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
   fence_after();
   const uint32_t tmem = tmem_base_s;
 
-  const int64_t items = (int64_t)g.mt * (g.dual == kDualM ? 2 : 1) * g.nt * g.splits;
+  const int64_t items = g.whole + (tiles_of(g) - g.whole) * g.splits;
   const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
   volatile int* const aborted = &abort_s;
 
@@ -464,19 +520,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
       commit<CG>(drained);
       wait_bar(drained, 0, kDrainNs);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 4 + 4 * kGroups) {
     // ---- epilogue
-    const int quad = warp & 3, half = (warp - 4) >> 2;
+    const int quad = warp & 3, part = (warp - 4) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     const EpiVec ev = epi_vec(g.ep);
     Piece pc;
     pc.smem = base + S::kStages * S::kStage + S::kBarBytes + (uint32_t)(warp - 4) * kStageBytes;
     pc.lane = lane;
-    const bool part_vec = runs_aligned(g.partial, g.n, 4) && (g.m * g.n) % 4 == 0;
+    const bool res_units = !kGated && g.ep.residual != nullptr && g.ep.out_type != kF32 && ev.res && g.n % 8 == 0;
     int buf = 0;
     uint32_t bph = 0;
     for (int64_t w = first; w < items; w += step) {
       const Item it = item_of(g, w);
+      const int64_t row0 = (int64_t)(it.mt * CG + (int)rank) * kRowsA + quad * 32, row = row0 + lane;
+      const bool inside = row < g.m;
+      auto place = [&](int c) {
+        pc.row0 = row0;
+        pc.col = (int64_t)it.nt * kTileN + c;
+        pc.rows = (int)max64(0, min64(32, g.m - row0));
+        pc.cols = (int)max64(0, min64(32, g.n - pc.col));
+      };
+      constexpr int kColsW = kTileN / kGroups;  // columns of a warp
+      uint4 res[4];
+      if (res_units) {
+        place(part * kColsW);
+        fetch_units(pc, g.ep.residual, g.ep.ldr * 2, res);
+      }
       if (*aborted || !wait_bar(tfull(buf), bph, kWaitNs)) {
         *aborted = 1;
         if (lane == 0) set_status(g_status, kTimeoutResult, (int)blockIdx.x, 2);
@@ -484,38 +554,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
       }
       __syncwarp();
       fence_after();
-      const int64_t row0 = (int64_t)(it.mt * CG + (int)rank) * kRowsA + quad * 32, row = row0 + lane;
-      const bool inside = row < g.m;
       const uint32_t acc = lanes + buf * NB;
 #pragma unroll 1
-      for (int c = half * (kTileN / 2); c < (half + 1) * (kTileN / 2); c += 32) {
-        const int64_t col = (int64_t)it.nt * kTileN + c;
-        if (row0 >= g.m || col >= g.n) break;  // the same for the whole warp
-        const int valid = inside ? (int)min64(32, g.n - col) : 0;
-        pc.row0 = row0;
-        pc.col = col;
-        pc.rows = (int)min64(32, g.m - row0);
-        pc.cols = (int)min64(32, g.n - col);
-        float v[32], u[kGated ? 32 : 1];
+      for (int c = part * kColsW; c < (part + 1) * kColsW; c += 32) {
+        place(c);
+        if (pc.rows <= 0 || pc.cols <= 0) break;  // the same for the whole warp
+        const int64_t col = pc.col;
+        const int valid = inside ? pc.cols : 0;
+        float v[32];
         tmem_load32(acc + c, v);
-        if constexpr (kGated) tmem_load32(acc + kTileN + c, u);
         tmem_load_wait();
-        if (g.splits > 1) {
-          float* p = g.partial + ((int64_t)it.split * (kGated || g.dual == kDualM ? 2 : 1) + it.prob) * g.m * g.n;
-          write_piece(pc, p, g.n, kF32, part_vec, v);
-          if constexpr (kGated) write_piece(pc, p + g.m * g.n, g.n, kF32, part_vec, u);
+        if (it.part >= 0) {
+          // this CTA's rows of the slot, all of them: the join looks at the sizes
+          Piece q = {pc.smem, (int64_t)((int)rank * kRowsA + quad * 32), c, 32, 32, lane};
+          float* p = g.partial + it.part * (CG * kRowsA * NB);
+          write_piece(q, p, NB, kF32, true, v);
+          if constexpr (kGated) {
+            tmem_load32(acc + kTileN + c, v);
+            tmem_load_wait();
+            q.col += kTileN;
+            write_piece(q, p, NB, kF32, true, v);
+          }
           continue;
         }
         epi_sums<32>(g.ep, ev, 0, inside ? row : 0, col, valid, v);
-        if constexpr (kGated) epi_sums<32>(g.ep, ev, 1, inside ? row : 0, col, valid, u);
-        if (g.ep.z_hi[0] != nullptr) {
-          write_kept(pc, g.ep.z_hi[0], g.ep.z_lo[0], g.ep.ldz, v);
-          if constexpr (kGated) write_kept(pc, g.ep.z_hi[1], g.ep.z_lo[1], g.ep.ldz, u);
+        if (g.ep.z_hi[0] != nullptr) write_kept(pc, g.ep.z_hi[0], g.ep.z_lo[0], g.ep.ldz, v);
+        if constexpr (kGated) {
+          float u[32];
+          tmem_load32(acc + kTileN + c, u);
+          act_run<32>(g.ep.act, v);
+          tmem_load_wait();
+          epi_sums<32>(g.ep, ev, 1, inside ? row : 0, col, valid, u);
+          if (g.ep.z_hi[1] != nullptr) write_kept(pc, g.ep.z_hi[1], g.ep.z_lo[1], g.ep.ldz, u);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= u[j];
+        } else {
+          if (res_units) {
+            act_run<32>(g.ep.act, v);
+            add_units(pc, res, g.ep.out_type, v);
+            if (c + 32 < (part + 1) * kColsW) {  // the next piece's, while this one is written
+              place(c + 32);
+              fetch_units(pc, g.ep.residual, g.ep.ldr * 2, res);
+              place(c);
+            }
+          } else {
+            epi_finish<32>(g.ep, ev, inside ? row : 0, col, valid, v);
+          }
         }
-        if constexpr (kGated)
-          epi_gate<32>(g.ep, v, u);
-        else
-          epi_finish<32>(g.ep, ev, inside ? row : 0, col, valid, v);
         write_piece(pc, g.ep.out[it.prob], g.ep.ldo, g.ep.out_type, ev.out, v);
       }
       fence_before();
@@ -534,28 +619,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm(const __grid_constant__ Ma
   if (warp == 2) tmem_free<CG>(tmem, S::kCols);
 }
 
-// Sum of the splits in their order, then the epilogue.  One thread takes 8
-// columns of one row.
+// Sum of a tile's pieces in their order, then the epilogue.  One thread takes 8
+// columns of one row; rows x nb: a slot of `partial`.
 template <bool kGated>
-__global__ void __launch_bounds__(256) k_join(Args g) {
-  const int64_t nc = (g.n + 7) / 8;
-  const int probs = g.dual == kDualM ? 2 : 1;
+__global__ void __launch_bounds__(256) k_join(const __grid_constant__ Args g, int rows, int nb) {
+  const int tile_n = kGated ? nb / 2 : nb, runs = tile_n / 8;
   const EpiVec ev = epi_vec(g.ep);
-  const bool vec = g.n % 4 == 0 && (g.m * g.n) % 4 == 0;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < nc * g.m * probs;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int prob = (int)(i / (nc * g.m));
-    const int64_t r = i - prob * nc * g.m, row = r / nc, col = (r - row * nc) * 8;
-    const int valid = (int)min64(8, g.n - col);
+  const int64_t total = (tiles_of(g) - g.whole) * rows * runs;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / runs;
+    const int c = (int)(i - r * runs) * 8;
+    const int64_t tile = r / rows;
+    const int rr = (int)(r - tile * rows);
+    Item it;
+    tile_of(g, g.whole + tile, it);
+    const int64_t row = (int64_t)it.mt * rows + rr, col = (int64_t)it.nt * tile_n + c;
+    if (row >= g.m || col >= g.n) continue;
     float v[8] = {}, u[8] = {};
-    for (int s = 0; s < g.splits; ++s) {
-      const float* p = g.partial + s * g.part_stride + prob * g.m * g.n;
+    const float* p = g.partial + tile * g.splits * rows * nb + (int64_t)rr * nb + c;
+    for (int s = 0; s < g.splits; ++s, p += (int64_t)rows * nb) {
       float t[8];
-      get_run<8>(p, row * g.n + col, kF32, valid, vec, t);
+      get_run<8>(p, 0, kF32, 8, true, t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += t[j];
       if (kGated) {
-        get_run<8>(p + g.m * g.n, row * g.n + col, kF32, valid, vec, t);
+        get_run<8>(p, tile_n, kF32, 8, true, t);
 #pragma unroll
         for (int j = 0; j < 8; ++j) u[j] += t[j];
       }
@@ -563,7 +651,7 @@ __global__ void __launch_bounds__(256) k_join(Args g) {
     if (kGated)
       epilogue_gated_run<8>(g.ep, ev, row, col, g.n, v, u);
     else
-      epilogue_run<8>(g.ep, ev, prob, row, col, g.n, v);
+      epilogue_run<8>(g.ep, ev, it.prob, row, col, g.n, v);
   }
 }
 
@@ -607,17 +695,18 @@ uint32_t make_idesc(const Gemm& g) {
          ((uint32_t)(g.major_b == kMajorMN) << 16) | ((uint32_t)(g.nb / 8) << 17) | ((uint32_t)(128 * g.cg / 16) << 24);
 }
 
-template <int CG, int NB, int MA, int MB, bool kFp8, bool kGated>
+template <int CG, int NB, int EW, int MA, int MB, bool kFp8, bool kGated>
 cudaError_t launch(const Maps& maps, const Args& args, int sms, cudaStream_t s) {
-  using S = Shape<CG, NB>;
-  auto* fn = &k_gemm<CG, NB, MA, MB, kFp8, kGated>;
+  using S = Shape<CG, NB, EW>;
+  auto* fn = &k_gemm<CG, NB, EW, MA, MB, kFp8, kGated>;
   // once a device; setting it again is harmless
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
-  const int64_t items = (int64_t)args.mt * (args.dual == kDualM ? 2 : 1) * args.nt * args.splits;
+  const int64_t tiles = (int64_t)args.mt * (args.dual == kDualM ? 2 : 1) * args.nt;
+  const int64_t items = args.whole + (tiles - args.whole) * args.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(items, sms / CG)));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -629,26 +718,35 @@ cudaError_t launch(const Maps& maps, const Args& args, int sms, cudaStream_t s) 
   return cudaLaunchKernelEx(&cfg, fn, maps, args);
 }
 
-template <int MA, int MB, bool kFp8, bool kGated>
+template <int EW, int MA, int MB, bool kFp8, bool kGated>
 cudaError_t launch_shape(const Gemm& g, const Maps& maps, const Args& args, int sms, cudaStream_t s) {
   if (g.cg == 2)
-    return g.nb == 256 ? launch<2, 256, MA, MB, kFp8, kGated>(maps, args, sms, s)
-                       : launch<2, 128, MA, MB, kFp8, kGated>(maps, args, sms, s);
-  return g.nb == 256 ? launch<1, 256, MA, MB, kFp8, kGated>(maps, args, sms, s)
-                     : launch<1, 128, MA, MB, kFp8, kGated>(maps, args, sms, s);
+    return g.nb == 256 ? launch<2, 256, EW, MA, MB, kFp8, kGated>(maps, args, sms, s)
+                       : launch<2, 128, EW, MA, MB, kFp8, kGated>(maps, args, sms, s);
+  return g.nb == 256 ? launch<1, 256, EW, MA, MB, kFp8, kGated>(maps, args, sms, s)
+                     : launch<1, 128, EW, MA, MB, kFp8, kGated>(maps, args, sms, s);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
-int64_t partial_floats(const Gemm& g) {
-  return g.splits > 1 ? (int64_t)g.splits * g.m * g.n * (g.dual == kDualN || g.dual == kDualM ? 2 : 1) : 0;
+namespace {
+int64_t tile_count(const Gemm& g) {
+  return ceil_div(g.m, kRowsA * g.cg) * (g.dual == kDualM ? 2 : 1) * ceil_div(g.n, g.dual == kDualN ? g.nb / 2 : g.nb);
+}
+// Tiles of the full waves; the rest is split where splits > 1.
+int64_t whole_tiles(const Gemm& g, int sms) {
+  const int64_t t = tile_count(g), slots = sms / g.cg;
+  return g.splits > 1 ? t / slots * slots : t;
+}
+int g_force[3] = {0, 0, 0};
+}  // namespace
+
+int64_t partial_floats(const Gemm& g, int sms) {
+  return (tile_count(g) - whole_tiles(g, sms)) * (g.splits > 1 ? g.splits : 0) * g.cg * kRowsA * g.nb;
 }
 
-namespace {
-int g_force[3] = {0, 0, 0};
-}
 void force_plan(int cg, int nb, int splits) {
   g_force[0] = cg;
   g_force[1] = nb;
@@ -662,31 +760,31 @@ void plan(Gemm& g, int sms, bool may_split) {
     g.splits = may_split ? g_force[2] : 1;
     return;
   }
-  // Time of a plan = waves of tiles x (k blocks x their time + a tile's fill and
-  // last epilogue) + the join of splits.  Microseconds a k block measured with
+  // Time of a plan = full waves of tiles x (k blocks x their time + a tile's fill)
+  // + what is behind them, in pieces of k where that fills the SMs + the last
+  // epilogue + the join of pieces.  Microseconds a k block measured with
   // 4096 x 4096 x 4096 and 8192 x 5632 x 2048: tiles of 128 columns read twice
   // the operand bytes a product and take 0.7 to 0.8 of the time of 256 columns,
   // so they win only where they fill the last wave.
   const int bk = g.type == kE4M3 ? 128 : 64;
   const int64_t kb = ceil_div(g.k, bk) * (g.dual == kDualK ? 2 : 1);
-  const int64_t outs = g.dual == kDualN || g.dual == kDualM ? 2 : 1;
   double best = 1e30;
-  for (int cg = 2; cg >= 1; --cg)
-    for (int nb = 256; nb >= 128; nb -= 128) {
-      const double t_kb = nb == 256 ? (cg == 2 ? 0.30 : 0.34) : (cg == 2 ? 0.23 : 0.235);
-      const int64_t tn = g.dual == kDualN ? nb / 2 : nb;
-      const int64_t tiles = ceil_div(g.m, 128 * cg) * ceil_div(g.n, tn) * (g.dual == kDualM ? 2 : 1);
-      const int64_t slots = sms / cg;
-      const int64_t most = may_split ? std::min<int64_t>(32, std::max<int64_t>(1, kb / 4)) : 1;
-      for (int64_t sp = 1; sp <= most; ++sp) {
-        if (sp > 1 && tiles * sp > 2 * slots) break;
-        const double join = sp > 1 ? 3.0 + (double)(sp + 1) * g.m * g.n * outs * 4 / 5e6 : 0.0;
-        const double t = ceil_div(tiles * sp, slots) * (ceil_div(kb, sp) * t_kb + 1.0) + join;
+  Gemm c = g;
+  for (c.cg = 2; c.cg >= 1; --c.cg)
+    for (c.nb = 256; c.nb >= 128; c.nb -= 128) {
+      const double t_kb = c.nb == 256 ? (c.cg == 2 ? 0.34 : 0.37) : (c.cg == 2 ? 0.26 : 0.27);
+      const int64_t slots = sms / c.cg, tiles = tile_count(c);
+      const int64_t full = tiles / slots, rest = tiles - full * slots;
+      const double wave = kb * t_kb + 0.7;
+      for (c.splits = 1; c.splits <= 32 && c.splits <= std::max<int64_t>(1, kb / 4); ++c.splits) {
+        if (c.splits > 1 && (!may_split || rest == 0 || rest * c.splits > slots)) break;
+        double t = full * wave + (rest ? ceil_div(kb, c.splits) * t_kb + 0.7 : 0.0) + c.nb / 64.0 * 0.6;
+        if (c.splits > 1) t += 4.0 + 2.0 * 4 * rest * c.splits * c.cg * kRowsA * c.nb / 5e6;
         if (t < best * 0.999) {
           best = t;
-          g.cg = cg;
-          g.nb = nb;
-          g.splits = (int)sp;
+          g.cg = c.cg;
+          g.nb = c.nb;
+          g.splits = c.splits;
         }
       }
     }
@@ -721,30 +819,34 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.kb = (int)ceil_div(g.k, bk);
   args.dual = g.dual;
   args.splits = g.splits;
+  args.whole = whole_tiles(g, sms);
   args.idesc = make_idesc(g);
-  args.part_stride = g.m * g.n * (gated || g.dual == kDualM ? 2 : 1);
   args.partial = g.partial;
   args.ep = g.ep;
+  // 16 k blocks take about as long as an epilogue with an activation
+  const bool busy = args.kb <= 16;
   if (g.type == kE4M3)
-    e = gated ? launch_shape<kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
-              : launch_shape<kMajorK, kMajorK, true, false>(g, maps, args, sms, s);
+    e = gated ? launch_shape<8, kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
+              : launch_shape<8, kMajorK, kMajorK, true, false>(g, maps, args, sms, s);
   else if (gated)
-    e = launch_shape<kMajorK, kMajorK, false, true>(g, maps, args, sms, s);
+    e = launch_shape<8, kMajorK, kMajorK, false, true>(g, maps, args, sms, s);
   else if (g.major_a == kMajorK && g.major_b == kMajorK)
-    e = launch_shape<kMajorK, kMajorK, false, false>(g, maps, args, sms, s);
+    e = busy ? launch_shape<16, kMajorK, kMajorK, false, false>(g, maps, args, sms, s)
+             : launch_shape<8, kMajorK, kMajorK, false, false>(g, maps, args, sms, s);
   else if (g.major_a == kMajorK)
-    e = launch_shape<kMajorK, kMajorMN, false, false>(g, maps, args, sms, s);
+    e = launch_shape<8, kMajorK, kMajorMN, false, false>(g, maps, args, sms, s);
   else if (g.major_b == kMajorMN)
-    e = launch_shape<kMajorMN, kMajorMN, false, false>(g, maps, args, sms, s);
+    e = launch_shape<8, kMajorMN, kMajorMN, false, false>(g, maps, args, sms, s);
   else
     return cudaErrorInvalidValue;
-  if (e != cudaSuccess || g.splits <= 1) return e;
-  const int64_t runs = ceil_div(g.n, 8) * g.m * (g.dual == kDualM ? 2 : 1);
+  const int64_t rest = tile_count(g) - args.whole;
+  if (e != cudaSuccess || rest == 0) return e;
+  const int64_t runs = rest * g.cg * kRowsA * tn / 8;
   const int grid = (int)std::min<int64_t>(ceil_div(runs, 256), (int64_t)sms * 8);
   if (gated)
-    k_join<true><<<grid, 256, 0, s>>>(args);
+    k_join<true><<<grid, 256, 0, s>>>(args, g.cg * kRowsA, g.nb);
   else
-    k_join<false><<<grid, 256, 0, s>>>(args);
+    k_join<false><<<grid, 256, 0, s>>>(args, g.cg * kRowsA, g.nb);
   return cudaGetLastError();
 }
 

@@ -265,13 +265,6 @@ __device__ __forceinline__ void epi_finish(const Epilogue& e, const EpiVec& ev, 
     for (int j = 0; j < C; ++j) v[j] += t[j];
   }
 }
-template <int C>
-__device__ __forceinline__ void epi_gate(const Epilogue& e, float (&g)[C], const float (&u)[C]) {
-  act_run<C>(e.act, g);
-#pragma unroll
-  for (int j = 0; j < C; ++j) g[j] *= u[j];
-}
-
 // All of it, stored by this thread.
 template <int C>
 __device__ __forceinline__ void epilogue_run(const Epilogue& e, const EpiVec& ev, int which, int64_t row, int64_t col,
@@ -292,7 +285,9 @@ __device__ __forceinline__ void epilogue_gated_run(const Epilogue& e, const EpiV
     put_kept<C>(e.z_hi[0], e.z_lo[0], row * e.ldz + col, valid, true, g);
     put_kept<C>(e.z_hi[1], e.z_lo[1], row * e.ldz + col, valid, true, u);
   }
-  epi_gate<C>(e, g, u);
+  act_run<C>(e.act, g);
+#pragma unroll
+  for (int j = 0; j < C; ++j) g[j] *= u[j];
   put_run<C>(e.out[0], row * e.ldo + col, e.out_type, valid, ev.out, g);
 }
 
