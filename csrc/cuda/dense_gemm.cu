@@ -55,6 +55,12 @@ __device__ __forceinline__ uint32_t cta_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// One lane of a warp whose 32 lanes are all here.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -63,22 +69,37 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+// kCluster: what the other CTA of a pair did before it arrived is to be seen.
+// That costs a fence of several hundred cycles, so the waits inside a tile, on
+// TMA's bytes and on finished products, go without (0.31 us a k block with it).
+template <bool kCluster>
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
+  if (kCluster)
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
   return ok != 0;
 }
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
-  if (try_wait_cluster(bar, parity)) return true;
+  if (try_wait<kCluster>(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
-  while (!try_wait_cluster(bar, parity))
+  while (!try_wait<kCluster>(bar, parity))
     if (globaltimer() - t0 > limit_ns) return false;
   return true;
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void arrive_leader(uint32_t bar) {
@@ -390,7 +411,11 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The warp's number in a uniform register: the loads' and products' warps run
+  // their loops as whole warps with uniform operands and elect a lane only to
+  // issue.  With one lane in a branch of its own each operand of each product is
+  // moved on its way (0.31 us a k block, whatever its size).
+  const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0u;
   if (threadIdx.x == 0) {
     abort_s = 0;
@@ -415,7 +440,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
   const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
   volatile int* const aborted = &abort_s;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     // ---- loads
     int s = 0;
     uint32_t ph = 0;
@@ -425,40 +450,41 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
       const Item it = item_of(g, w);
       const int row_a = (it.mt * CG + (int)rank) * kRowsA;
       for (int kb = it.k0; kb < it.k1; ++kb) {
-        if (*aborted || !wait_bar(empty(s), ph ^ 1u, kWaitNs)) {
-          ok = false;
-          break;
-        }
-        if (rank == 0) mbar_expect_tx(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(full(s))), CG * S::kStage);
+        ok = __all_sync(kFull, *aborted == 0 && wait_bar(empty(s), ph ^ 1u, kWaitNs));
+        if (!ok) break;
         const uint32_t bar = CG == 2 ? map_to_rank(full(s), 0) : full(s);
         const int seg = g.dual == kDualK && kb >= g.kb ? 1 : 0;
         const int k = (kb - seg * g.kb) * kBk;
         const CUtensorMap* ma = &maps.a[g.dual == kDualM ? it.prob : seg];
+        const CUtensorMap* mb = &maps.b[seg];
         const uint32_t da = base + s * S::kStage, db = da + S::kBytesA;
-        if (MA == kMajorK) {
-          tma_load<CG>(da, ma, k, row_a, bar);
-        } else {
-#pragma unroll
-          for (int c = 0; c < kRowsA / 64; ++c) tma_load<CG>(da + c * 8192, ma, row_a + 64 * c, k, bar);
-        }
-        if (kGated) {
-          // gate rows in the accumulator's first half, up rows in its second
-          if (CG == 2) {
-            tma_load<CG>(db, &maps.b[rank], k, it.nt * kTileN, bar);
-          } else {
-            tma_load<CG>(db, &maps.b[0], k, it.nt * kTileN, bar);
-            tma_load<CG>(db + S::kBytesB / 2, &maps.b[1], k, it.nt * kTileN, bar);
-          }
-        } else {
-          const CUtensorMap* mb = &maps.b[seg];
-          const int row_b = it.nt * NB + (int)rank * S::kRowsB;
-          if (MB == kMajorK) {
-            tma_load<CG>(db, mb, k, row_b, bar);
+        if (elect_one()) {
+          if (rank == 0) expect_bytes(full(s), CG * S::kStage);
+          if (MA == kMajorK) {
+            tma_load<CG>(da, ma, k, row_a, bar);
           } else {
 #pragma unroll
-            for (int c = 0; c < S::kRowsB / 64; ++c) tma_load<CG>(db + c * 8192, mb, row_b + 64 * c, k, bar);
+            for (int c = 0; c < kRowsA / 64; ++c) tma_load<CG>(da + c * 8192, ma, row_a + 64 * c, k, bar);
+          }
+          if (kGated) {
+            // gate rows in the accumulator's first half, up rows in its second
+            if (CG == 2) {
+              tma_load<CG>(db, &maps.b[rank], k, it.nt * kTileN, bar);
+            } else {
+              tma_load<CG>(db, &maps.b[0], k, it.nt * kTileN, bar);
+              tma_load<CG>(db + S::kBytesB / 2, &maps.b[1], k, it.nt * kTileN, bar);
+            }
+          } else {
+            const int row_b = it.nt * NB + (int)rank * S::kRowsB;
+            if (MB == kMajorK) {
+              tma_load<CG>(db, mb, k, row_b, bar);
+            } else {
+#pragma unroll
+              for (int c = 0; c < S::kRowsB / 64; ++c) tma_load<CG>(db + c * 8192, mb, row_b + 64 * c, k, bar);
+            }
           }
         }
+        __syncwarp();
         ++loads;
         if (++s == S::kStages) {
           s = 0;
@@ -468,7 +494,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     }
     if (!ok) {
       *aborted = 1;
-      set_status(g_status, kTimeoutCopy, (int)blockIdx.x, 0);
+      if (lane == 0) set_status(g_status, kTimeoutCopy, (int)blockIdx.x, 0);
       // copies in flight land before the shared memory is given up
       if (rank == 0) {
         const int64_t from = loads > S::kStages ? loads - S::kStages : 0;
@@ -476,39 +502,41 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
           wait_bar(full((int)(l % S::kStages)), (uint32_t)((l / S::kStages) & 1), kDrainNs);
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     // ---- products
     int s = 0;
     uint32_t ph = 0;
     int buf = 0;
     uint32_t bph = 0;
     bool ok = true;
+    const uint64_t desc_a = smem_desc<MA>(base), desc_b = smem_desc<MB>(base + S::kBytesA);
     for (int64_t w = first; ok && w < items; w += step) {
       const Item it = item_of(g, w);
-      if (*aborted || !wait_bar(tempty(buf), bph ^ 1u, kWaitNs)) {
-        ok = false;
-        break;
-      }
+      ok = __all_sync(kFull, *aborted == 0 && wait_bar<CG == 2>(tempty(buf), bph ^ 1u, kWaitNs));
+      if (!ok) break;
       fence_after();
       const uint32_t d = tmem + buf * NB;
       for (int kb = it.k0; kb < it.k1; ++kb) {
-        if (!wait_bar(full(s), ph, kWaitNs)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(kFull, wait_bar(full(s), ph, kWaitNs));
+        if (!ok) break;
         fence_after();
-        const uint32_t sa = base + s * S::kStage, sb = sa + S::kBytesA;
+        // addresses are the low bits of a descriptor, in units of 16 bytes
+        const uint64_t sa = desc_a + (uint64_t)(s * (S::kStage >> 4)), sb = desc_b + (uint64_t)(s * (S::kStage >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma<CG, kFp8>(d, smem_desc<MA>(sa + j * kStep<MA>), smem_desc<MB>(sb + j * kStep<MB>), g.idesc,
-                        (kb > it.k0 || j > 0) ? 1u : 0u);
-        commit<CG>(empty(s));
+          for (int j = 0; j < 4; ++j)
+            mma<CG, kFp8>(d, sa + j * (kStep<MA> >> 4), sb + j * (kStep<MB> >> 4), g.idesc,
+                          (kb > it.k0 || j > 0) ? 1u : 0u);
+          commit<CG>(empty(s));
+        }
+        __syncwarp();
         if (++s == S::kStages) {
           s = 0;
           ph ^= 1u;
         }
       }
-      commit<CG>(tfull(buf));
+      if (elect_one()) commit<CG>(tfull(buf));
+      __syncwarp();
       if (++buf == 2) {
         buf = 0;
         bph ^= 1u;
@@ -516,8 +544,9 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     }
     if (!ok) {
       *aborted = 1;
-      set_status(g_status, kTimeoutPayload, (int)blockIdx.x, 1);
-      commit<CG>(drained);
+      if (lane == 0) set_status(g_status, kTimeoutPayload, (int)blockIdx.x, 1);
+      if (elect_one()) commit<CG>(drained);
+      __syncwarp();
       wait_bar(drained, 0, kDrainNs);
     }
   } else if (warp >= 4 && warp < 4 + 4 * kGroups) {
