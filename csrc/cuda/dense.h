@@ -57,8 +57,8 @@ struct Gemm {
   int dual;
   Operand a[2], b[2];
   Epilogue ep;
-  float* partial;  // partial_floats(): sums of the tiles that are split
-  int splits;      // pieces of k of each tile behind the last full wave
+  float* partial;  // partial_floats(): sums of the pieces of k, when splits > 1
+  int splits;
   int cg, nb;      // CTAs per tile (1 or 2), accumulator columns of a tile
 };
 
@@ -68,7 +68,7 @@ void plan(Gemm& g, int sms, bool may_split);
 // Every following product takes this plan (tests and measurements of one tile
 // shape); cg = 0 returns to plan().
 void force_plan(int cg, int nb, int splits);
-int64_t partial_floats(const Gemm& g, int sms);
+int64_t partial_floats(const Gemm& g);
 
 // Enqueue the product.  Every operand must be fit for TMA: base 16-byte
 // aligned, row stride a multiple of 16 bytes (ld_fits).  Returns a CUDA

@@ -28,7 +28,7 @@ void run_gemm(Gemm& g, const torch::Tensor& like, std::vector<torch::Tensor>& ke
   const int sms = sm_count(like.get_device());
   plan(g, sms, true);
   g.partial = nullptr;
-  if (const int64_t f = partial_floats(g, sms)) {
+  if (const int64_t f = partial_floats(g)) {
     keep.push_back(torch::empty({f}, like.options().dtype(torch::kFloat32)));
     g.partial = keep.back().data_ptr<float>();
   }

@@ -42,10 +42,9 @@ struct Args {
   int mt, nt;        // tiles of one problem along m and n
   int kb;            // k blocks of one operand pair
   int dual;
-  int64_t whole;     // tiles summed in one piece; those behind them in `splits` pieces
-  int splits;
+  int splits;        // pieces of k of each tile
   uint32_t idesc;
-  float* partial;    // [split tiles, splits, rows of a tile, NB] sums
+  float* partial;    // [tiles, splits, rows of a tile, NB] sums, where splits > 1
   Epilogue ep;
 };
 
@@ -357,40 +356,42 @@ struct Item {
   int prob;     // kDualM: which product
   int mt, nt;   // tile
   int k0, k1;   // k blocks
-  int64_t part; // slot of `partial`, or -1
+  int part;     // slot of `partial`, or -1
 };
-__device__ __forceinline__ int64_t tiles_of(const Args& g) {
-  return (int64_t)g.mt * (g.dual == kDualM ? 2 : 1) * g.nt;
+__device__ __forceinline__ uint32_t tiles_of(const Args& g) {
+  return (uint32_t)g.mt * (g.dual == kDualM ? 2u : 1u) * (uint32_t)g.nt;
 }
 // Tile t.  Groups of 8 rows of tiles sweep the columns together, so that the
-// tiles that run at one time share their operands in L2.
-__device__ __forceinline__ void tile_of(const Args& g, int64_t t, Item& it) {
-  const int rows = g.mt * (g.dual == kDualM ? 2 : 1);
-  const int64_t per = 8ll * g.nt;
-  const int grp = (int)(t / per), in = (int)(t - grp * per);
-  const int h = min(8, rows - grp * 8);
-  it.nt = in / h;
-  const int r = grp * 8 + in % h;
-  it.prob = r / g.mt;
-  it.mt = r - it.prob * g.mt;
+// tiles that run at one time share their operands in L2.  32-bit arithmetic: the
+// host refuses more tiles, and every warp divides once a tile.
+__device__ __forceinline__ void tile_of(const Args& g, uint32_t t, Item& it) {
+  const uint32_t rows = (uint32_t)g.mt * (g.dual == kDualM ? 2u : 1u);
+  const uint32_t per = 8u * (uint32_t)g.nt;
+  const uint32_t grp = t / per, in = t - grp * per;
+  const uint32_t h = min(8u, rows - grp * 8u);
+  const uint32_t nt = h == 8u ? in >> 3 : in / h;
+  const uint32_t r = grp * 8u + (in - nt * h);
+  it.nt = (int)nt;
+  it.prob = r >= (uint32_t)g.mt ? 1 : 0;
+  it.mt = (int)r - it.prob * g.mt;
 }
-// Work item w: a whole tile, or one of the pieces of k of a tile behind them.
-__device__ __forceinline__ Item item_of(const Args& g, int64_t w) {
+// Work item w: a tile, or one of its pieces of k.
+__device__ __forceinline__ Item item_of(const Args& g, uint32_t w) {
   Item it;
   const int kb = g.kb * (g.dual == kDualK ? 2 : 1);
-  if (w < g.whole) {
+  if (g.splits == 1) {
     tile_of(g, w, it);
     it.k0 = 0;
     it.k1 = kb;
     it.part = -1;
     return it;
   }
-  it.part = w - g.whole;
-  const int64_t r = it.part / g.splits;
-  const int sp = (int)(it.part - r * g.splits);
-  tile_of(g, g.whole + r, it);
+  const uint32_t t = w / (uint32_t)g.splits;
+  const int sp = (int)(w - t * (uint32_t)g.splits);
+  tile_of(g, t, it);
   it.k0 = (int)((int64_t)kb * sp / g.splits);
   it.k1 = (int)((int64_t)kb * (sp + 1) / g.splits);
+  it.part = (int)w;
   return it;
 }
 
@@ -436,8 +437,8 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
   fence_after();
   const uint32_t tmem = tmem_base_s;
 
-  const int64_t items = g.whole + (tiles_of(g) - g.whole) * g.splits;
-  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const uint32_t items = tiles_of(g) * (uint32_t)g.splits;
+  const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
   volatile int* const aborted = &abort_s;
 
   if (warp == 0) {
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     uint32_t ph = 0;
     int64_t loads = 0;
     bool ok = true;
-    for (int64_t w = first; ok && w < items; w += step) {
+    for (uint32_t w = first; ok && w < items; w += step) {
       const Item it = item_of(g, w);
       const int row_a = (it.mt * CG + (int)rank) * kRowsA;
       for (int kb = it.k0; kb < it.k1; ++kb) {
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     uint32_t bph = 0;
     bool ok = true;
     const uint64_t desc_a = smem_desc<MA>(base), desc_b = smem_desc<MB>(base + S::kBytesA);
-    for (int64_t w = first; ok && w < items; w += step) {
+    for (uint32_t w = first; ok && w < items; w += step) {
       const Item it = item_of(g, w);
       ok = __all_sync(kFull, *aborted == 0 && wait_bar<CG == 2>(tempty(buf), bph ^ 1u, kWaitNs));
       if (!ok) break;
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     const bool res_units = !kGated && g.ep.residual != nullptr && g.ep.out_type != kF32 && ev.res && g.n % 8 == 0;
     int buf = 0;
     uint32_t bph = 0;
-    for (int64_t w = first; w < items; w += step) {
+    for (uint32_t w = first; w < items; w += step) {
       const Item it = item_of(g, w);
       const int64_t row0 = (int64_t)(it.mt * CG + (int)rank) * kRowsA + quad * 32, row = row0 + lane;
       const bool inside = row < g.m;
@@ -596,7 +597,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
         if (it.part >= 0) {
           // this CTA's rows of the slot, all of them: the join looks at the sizes
           Piece q = {pc.smem, (int64_t)((int)rank * kRowsA + quad * 32), c, 32, 32, lane};
-          float* p = g.partial + it.part * (CG * kRowsA * NB);
+          float* p = g.partial + (int64_t)it.part * (CG * kRowsA * NB);
           write_piece(q, p, NB, kF32, true, v);
           if constexpr (kGated) {
             tmem_load32(acc + kTileN + c, v);
@@ -654,14 +655,14 @@ template <bool kGated>
 __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Args g, int rows, int nb) {
   const int tile_n = kGated ? nb / 2 : nb, runs = tile_n / 8;
   const EpiVec ev = epi_vec(g.ep);
-  const int64_t total = (tiles_of(g) - g.whole) * rows * runs;
+  const int64_t total = (int64_t)tiles_of(g) * rows * runs;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / runs;
     const int c = (int)(i - r * runs) * 8;
     const int64_t tile = r / rows;
     const int rr = (int)(r - tile * rows);
     Item it;
-    tile_of(g, g.whole + tile, it);
+    tile_of(g, (uint32_t)tile, it);
     const int64_t row = (int64_t)it.mt * rows + rr, col = (int64_t)it.nt * tile_n + c;
     if (row >= g.m || col >= g.n) continue;
     float v[8] = {}, u[8] = {};
@@ -732,7 +733,7 @@ cudaError_t launch(const Maps& maps, const Args& args, int sms, cudaStream_t s) 
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t tiles = (int64_t)args.mt * (args.dual == kDualM ? 2 : 1) * args.nt;
-  const int64_t items = args.whole + (tiles - args.whole) * args.splits;
+  const int64_t items = tiles * args.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(items, sms / CG)));
   cfg.blockDim = dim3(S::kThreads);
@@ -764,16 +765,11 @@ namespace {
 int64_t tile_count(const Gemm& g) {
   return ceil_div(g.m, kRowsA * g.cg) * (g.dual == kDualM ? 2 : 1) * ceil_div(g.n, g.dual == kDualN ? g.nb / 2 : g.nb);
 }
-// Tiles of the full waves; the rest is split where splits > 1.
-int64_t whole_tiles(const Gemm& g, int sms) {
-  const int64_t t = tile_count(g), slots = sms / g.cg;
-  return g.splits > 1 ? t / slots * slots : t;
-}
 int g_force[3] = {0, 0, 0};
 }  // namespace
 
-int64_t partial_floats(const Gemm& g, int sms) {
-  return (tile_count(g) - whole_tiles(g, sms)) * (g.splits > 1 ? g.splits : 0) * g.cg * kRowsA * g.nb;
+int64_t partial_floats(const Gemm& g) {
+  return g.splits > 1 ? tile_count(g) * g.splits * g.cg * kRowsA * g.nb : 0;
 }
 
 void force_plan(int cg, int nb, int splits) {
@@ -789,26 +785,30 @@ void plan(Gemm& g, int sms, bool may_split) {
     g.splits = may_split ? g_force[2] : 1;
     return;
   }
-  // Time of a plan = full waves of tiles x (k blocks x their time + a tile's fill)
-  // + what is behind them, in pieces of k where that fills the SMs + the last
-  // epilogue + the join of pieces.  Microseconds a k block measured with
-  // 4096 x 4096 x 4096 and 8192 x 5632 x 2048: tiles of 128 columns read twice
-  // the operand bytes a product and take 0.7 to 0.8 of the time of 256 columns,
-  // so they win only where they fill the last wave.
+  // Time of a plan = waves of tiles x the longer of their products and their
+  // epilogue + the first fill and the last epilogue + the join of pieces of k.
+  // Microseconds of a k block and of an epilogue as measured on a busy GPU with
+  // 8192 x 5632 x 2048 and 8192 x 2048 x 256: tiles of 128 columns take 0.6 of
+  // the time of 256 columns for half of the work, so they win where they fill
+  // the last wave, or where the epilogue rules; a pair of CTAs saves a third of
+  // the operand bytes, but its epilogues wait for one another.  The join is a
+  // launch of its own (128 x 5632 x 2048 in three pieces: 18 us, whole: 12), so
+  // k is split only where tiles leave most SMs idle.  Splitting the tiles behind
+  // the last full wave gained nothing: a busy GPU runs at its power limit, and a
+  // wave half empty at a higher clock.
   const int bk = g.type == kE4M3 ? 128 : 64;
   const int64_t kb = ceil_div(g.k, bk) * (g.dual == kDualK ? 2 : 1);
   double best = 1e30;
   Gemm c = g;
   for (c.cg = 2; c.cg >= 1; --c.cg)
     for (c.nb = 256; c.nb >= 128; c.nb -= 128) {
-      const double t_kb = c.nb == 256 ? (c.cg == 2 ? 0.34 : 0.37) : (c.cg == 2 ? 0.26 : 0.27);
+      const double t_kb = c.nb == 256 ? (c.cg == 2 ? 0.36 : 0.39) : (c.cg == 2 ? 0.23 : 0.24);
+      const double t_epi = c.nb == 256 ? (c.cg == 2 ? 5.2 : 3.6) : (c.cg == 2 ? 3.0 : 2.1);
       const int64_t slots = sms / c.cg, tiles = tile_count(c);
-      const int64_t full = tiles / slots, rest = tiles - full * slots;
-      const double wave = kb * t_kb + 0.7;
       for (c.splits = 1; c.splits <= 32 && c.splits <= std::max<int64_t>(1, kb / 4); ++c.splits) {
-        if (c.splits > 1 && (!may_split || rest == 0 || rest * c.splits > slots)) break;
-        double t = full * wave + (rest ? ceil_div(kb, c.splits) * t_kb + 0.7 : 0.0) + c.nb / 64.0 * 0.6;
-        if (c.splits > 1) t += 4.0 + 2.0 * 4 * rest * c.splits * c.cg * kRowsA * c.nb / 5e6;
+        if (c.splits > 1 && (!may_split || tiles * c.splits > slots)) break;
+        double t = ceil_div(tiles * c.splits, slots) * std::max(ceil_div(kb, c.splits) * t_kb + 0.3, t_epi) + t_epi;
+        if (c.splits > 1) t += 6.0 + 2.0 * 4 * tiles * c.splits * c.cg * kRowsA * c.nb / 5e6;
         if (t < best * 0.999) {
           best = t;
           g.cg = c.cg;
@@ -821,6 +821,7 @@ void plan(Gemm& g, int sms, bool may_split) {
 
 cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   if (g.m <= 0 || g.n <= 0 || g.k <= 0) return cudaErrorInvalidValue;
+  if (tile_count(g) * g.splits >= (int64_t(1) << 30)) return cudaErrorInvalidValue;  // 2^44 outputs
   if (encoder() == nullptr) return cudaErrorNotSupported;
   // The encoder is a driver call and needs a current context, which a thread
   // of autograd's may not have yet: setting the device makes it current.
@@ -848,7 +849,6 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.kb = (int)ceil_div(g.k, bk);
   args.dual = g.dual;
   args.splits = g.splits;
-  args.whole = whole_tiles(g, sms);
   args.idesc = make_idesc(g);
   args.partial = g.partial;
   args.ep = g.ep;
@@ -868,9 +868,8 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
     e = launch_shape<8, kMajorMN, kMajorMN, false, false>(g, maps, args, sms, s);
   else
     return cudaErrorInvalidValue;
-  const int64_t rest = tile_count(g) - args.whole;
-  if (e != cudaSuccess || rest == 0) return e;
-  const int64_t runs = rest * g.cg * kRowsA * tn / 8;
+  if (e != cudaSuccess || g.splits == 1) return e;
+  const int64_t runs = tile_count(g) * g.cg * kRowsA * tn / 8;
   const int grid = (int)std::min<int64_t>(ceil_div(runs, 256), (int64_t)sms * 8);
   if (gated)
     k_join<true><<<grid, 256, 0, s>>>(args, g.cg * kRowsA, g.nb);
