@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "dense_math.cuh"
+#include "layer_launch.cuh"
 #include "ngl_cuda.cuh"
 
 namespace ngl {
@@ -26,6 +27,8 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_act_backward(const void* d
                                                                    const uint16_t* z_hi, const uint8_t* z_lo,
                                                                    int half_type, int64_t m, int64_t n, void* dz,
                                                                    float* partial) {
+  pdl_begin();
+  pdl_wait();
   const int64_t col = ((int64_t)blockIdx.x * kLanesX + threadIdx.x) * kColGroup;
   const int valid = (int)max64(0, min64(kColGroup, n - col));
   const bool vdy = runs_aligned(dy, ldy, type_bytes(dy_type)), vo = runs_aligned(dz, n, 2);
@@ -68,6 +71,8 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_act_backward(const void* d
 // Column sums of [parts, n]: 32 columns a CTA, 32 threads along the parts, joined in their order.
 constexpr int kSumY = 32;
 __global__ void __launch_bounds__(32 * kSumY) k_colsum(const float* partial, int parts, int64_t n, void* out, int type) {
+  pdl_begin();
+  pdl_wait();
   __shared__ float s[kSumY][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float a = 0.0f;
@@ -90,6 +95,8 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_gated_backward(const void*
                                                                      const uint8_t* g_lo, const uint16_t* u_hi,
                                                                      const uint8_t* u_lo, int half_type, int64_t m,
                                                                      int64_t n, void* dg, void* du) {
+  pdl_begin();
+  pdl_wait();
   const int64_t col = ((int64_t)blockIdx.x * kLanesX + threadIdx.x) * kColGroup;
   const int valid = (int)max64(0, min64(kColGroup, n - col));
   if (valid <= 0) return;
@@ -120,6 +127,8 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_gated_backward(const void*
 template <typename T>
 __global__ void __launch_bounds__(256) k_repack(const T* src, int64_t lds, T* dst, int64_t ldd, int64_t rows,
                                                 int64_t cols) {
+  pdl_begin();
+  pdl_wait();
   const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (c >= ldd) return;  // ldd is a multiple of 8
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
@@ -154,8 +163,8 @@ int row_ctas(int64_t m, int64_t n, int sms) {
 int colsum_parts(int64_t m, int64_t n, int sms) { return row_ctas(m, n, sms); }
 
 cudaError_t colsum(const float* partial, int parts, int64_t n, void* out, int type, cudaStream_t s) {
-  k_colsum<<<(unsigned)((n + 31) / 32), dim3(32, kSumY), 0, s>>>(partial, parts, n, out, type);
-  return cudaGetLastError();
+  return launch_dependent(&k_colsum, dim3((unsigned)((n + 31) / 32)), dim3(32, kSumY), 0, 1, s, partial, parts, n, out,
+                          type);
 }
 
 cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_t* z_hi, const uint8_t* z_lo, int act,
@@ -164,11 +173,11 @@ cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)parts);
 #define NGL_CALL(a)                                                                                          \
-  k_act_backward<a><<<grid, dim3(kLanesX, kLanesY), 0, s>>>(dy, dy_type, ldy, z_hi, z_lo, half_type, m, n, dz, \
-                                                            db != nullptr ? partial : nullptr)
+  e = launch_dependent(&k_act_backward<a>, grid, dim3(kLanesX, kLanesY), 0, 1, s, dy, dy_type, ldy, z_hi, z_lo, \
+                       half_type, m, n, dz, db != nullptr ? partial : nullptr)
+  cudaError_t e = cudaSuccess;
   NGL_BY_ACT(NGL_CALL)
 #undef NGL_CALL
-  const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess || db == nullptr ? e : colsum(partial, parts, n, db, half_type, s);
 }
 
@@ -177,11 +186,12 @@ cudaError_t gated_backward(const void* dh, int64_t ldh, const uint16_t* const z_
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)row_ctas(m, n, sms));
 #define NGL_CALL(a)                                                                                             \
-  k_gated_backward<a><<<grid, dim3(kLanesX, kLanesY), 0, s>>>(dh, ldh, z_hi[0], z_lo[0], z_hi[1], z_lo[1], half_type, \
-                                                              m, n, dg, du)
+  e = launch_dependent(&k_gated_backward<a>, grid, dim3(kLanesX, kLanesY), 0, 1, s, dh, ldh, z_hi[0], z_lo[0], \
+                       z_hi[1], z_lo[1], half_type, m, n, dg, du)
+  cudaError_t e = cudaSuccess;
   NGL_BY_ACT(NGL_CALL)
 #undef NGL_CALL
-  return cudaGetLastError();
+  return e;
 }
 
 cudaError_t repack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int elem,
@@ -189,12 +199,10 @@ cudaError_t repack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t
   if (rows <= 0 || cols <= 0) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((ldd + 2047) / 2048), (unsigned)std::min<int64_t>(rows, 65535));
   if (elem == 1)
-    k_repack<uint8_t><<<grid, 256, 0, s>>>(static_cast<const uint8_t*>(src), lds, static_cast<uint8_t*>(dst), ldd,
-                                           rows, cols);
-  else
-    k_repack<uint16_t><<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(src), lds, static_cast<uint16_t*>(dst), ldd,
-                                            rows, cols);
-  return cudaGetLastError();
+    return launch_dependent(&k_repack<uint8_t>, grid, dim3(256), 0, 1, s, static_cast<const uint8_t*>(src), lds,
+                            static_cast<uint8_t*>(dst), ldd, rows, cols);
+  return launch_dependent(&k_repack<uint16_t>, grid, dim3(256), 0, 1, s, static_cast<const uint16_t*>(src), lds,
+                          static_cast<uint16_t*>(dst), ldd, rows, cols);
 }
 
 }  // namespace dense

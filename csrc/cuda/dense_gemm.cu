@@ -18,6 +18,7 @@
 #include <cstring>
 
 #include "dense_math.cuh"
+#include "layer_launch.cuh"
 #include "ngl_cuda.cuh"
 
 namespace ngl {
@@ -416,6 +417,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
   // their loops as whole warps with uniform operands and elect a lane only to
   // issue.  With one lane in a branch of its own each operand of each product is
   // moved on its way (0.31 us a k block, whatever its size).
+  pdl_begin();
   const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cta_rank() : 0u;
   if (threadIdx.x == 0) {
@@ -436,6 +438,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
   if (CG == 2) cluster_sync(); else __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_base_s;
+  pdl_wait();
 
   const uint32_t items = tiles_of(g) * (uint32_t)g.splits;
   const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
@@ -653,6 +656,8 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
 // columns of one row; rows x nb: a slot of `partial`.
 template <bool kGated>
 __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Args g, int rows, int nb) {
+  pdl_begin();
+  pdl_wait();
   const int tile_n = kGated ? nb / 2 : nb, runs = tile_n / 8;
   const EpiVec ev = epi_vec(g.ep);
   const int64_t total = (int64_t)tiles_of(g) * rows * runs;
@@ -734,18 +739,8 @@ cudaError_t launch(const Maps& maps, const Args& args, int sms, cudaStream_t s) 
   if (e != cudaSuccess) return e;
   const int64_t tiles = (int64_t)args.mt * (args.dual == kDualM ? 2 : 1) * args.nt;
   const int64_t items = tiles * args.splits;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(items, sms / CG)));
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, maps, args);
+  return launch_dependent(fn, dim3((unsigned)(CG * std::min<int64_t>(items, sms / CG))), dim3(S::kThreads), S::kSmem, CG,
+                          s, maps, args);
 }
 
 template <int EW, int MA, int MB, bool kFp8, bool kGated>
@@ -871,11 +866,8 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   if (e != cudaSuccess || g.splits == 1) return e;
   const int64_t runs = tile_count(g) * g.cg * kRowsA * tn / 8;
   const int grid = (int)std::min<int64_t>(ceil_div(runs, 256), (int64_t)sms * 8);
-  if (gated)
-    k_join<true><<<grid, 256, 0, s>>>(args, g.cg * kRowsA, g.nb);
-  else
-    k_join<false><<<grid, 256, 0, s>>>(args, g.cg * kRowsA, g.nb);
-  return cudaGetLastError();
+  return launch_dependent(gated ? &k_join<true> : &k_join<false>, dim3(grid), dim3(256), 0, 1, s, args,
+                          g.cg * kRowsA, g.nb);
 }
 
 cudaError_t read_status(int* out4, bool clear, cudaStream_t s) {

@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "dense_math.cuh"
+#include "layer_launch.cuh"
 #include "ngl_cuda.cuh"
 
 namespace ngl {
@@ -78,6 +79,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
 // bytes.  Rows beyond the last are read as the last: their sums go nowhere.
 template <int NT, int U, bool kHigh, bool kGated, bool kFp8, bool kVec>
 __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ Skinny g) {
+  pdl_begin();
   constexpr int NW = kGated ? 2 : 1;
   constexpr int elem = kFp8 ? 1 : 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -101,6 +103,18 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[w][n][i] = 0.0f;
 
+  // The CTA's weights on their way into L2 while the kernel before this one ends
+  // (L2 is where all writes meet, so whatever it writes is still seen).
+  if (kVec && warp == 0 && lane < 8 * NT * NW) {
+    const int64_t row = j0 + lane % (8 * NT);
+    const int w = lane / (8 * NT);
+    if (row < g.n)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const uint8_t*>(g.w[w].p) +
+                                                                    row * g.w[w].ld * elem),
+                   "r"((uint32_t)min64(kbytes, 1 << 16))
+                   : "memory");
+  }
+  pdl_wait();
   for (int64_t b0 = (int64_t)warp * (U * 64); b0 < kbytes; b0 += kWarps * U * 64) {
     uint4 wv[U][NW][NT], xa[U], xb[U];
     if (kVec && b0 + U * 64 <= kbytes) {
@@ -217,11 +231,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
 template <int NT, int U, bool kHigh, bool kGated, bool kFp8>
 cudaError_t launch_nt(const Skinny& g, bool vec, cudaStream_t s) {
   const unsigned grid = (unsigned)((g.n + 8 * NT - 1) / (8 * NT));
-  if (vec)
-    k_skinny<NT, U, kHigh, kGated, kFp8, true><<<grid, kWarps * 32, 0, s>>>(g);
-  else
-    k_skinny<NT, 2, kHigh, kGated, kFp8, false><<<grid, kWarps * 32, 0, s>>>(g);
-  return cudaGetLastError();
+  return launch_dependent(
+      vec ? &k_skinny<NT, U, kHigh, kGated, kFp8, true> : &k_skinny<NT, 2, kHigh, kGated, kFp8, false>, dim3(grid),
+      dim3(kWarps * 32), 0, 1, s, g);
 }
 // 8 loads of weights in flight a thread.
 template <bool kGated, bool kFp8>

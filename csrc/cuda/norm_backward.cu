@@ -19,6 +19,8 @@ constexpr int back_ctas(int tpr) { return tpr > 256 ? 1 : 2; }
 
 template <int XT, int ST, int TPR, int VPT, bool kVec>
 __global__ void __launch_bounds__(kBackCta<TPR>, back_ctas(TPR)) k_backward(const __grid_constant__ Backward b) {
+  pdl_begin();
+  pdl_wait();
   constexpr int kGroups = kBackCta<TPR> / TPR;
   __shared__ float sm[kGroups][4 * (TPR / 32)];
   extern __shared__ float dw_sm[];  // [width], where kGroups > 1
@@ -124,8 +126,7 @@ cudaError_t run_backward(const Backward& b, cudaStream_t st) {
   auto* fn = vec ? &k_backward<XT, ST, TPR, VPT, true> : &k_backward<XT, ST, TPR, VPT, false>;
   // at most 16 KB: several groups only up to rows of 4096 elements
   const int smem = b.partial != nullptr && kBackCta<TPR> / TPR > 1 ? (int)b.width * 4 : 0;
-  fn<<<b.parts, kBackCta<TPR>, smem, st>>>(b);
-  return cudaGetLastError();
+  return launch_dependent(fn, dim3((unsigned)b.parts), dim3(kBackCta<TPR>), smem, 1, st, b);
 }
 template <int XT, int ST>
 cudaError_t backward_of(const Backward& p, cudaStream_t st) {

@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "dense_math.cuh"
+#include "layer_launch.cuh"
 #include "ngl_cuda.cuh"
 
 namespace ngl {

@@ -20,6 +20,8 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 
 template <int XT, int ST, int TPR, int VPT, bool kFp8, bool kVec>
 __global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ Forward f) {
+  pdl_begin();
+  pdl_wait();
   constexpr int kRows = kCta<TPR> / TPR;
   __shared__ float sm[kRows][2 * (TPR / 32)];
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, width = (int)f.width;
@@ -122,8 +124,8 @@ cudaError_t start(const Forward& f, int sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
   }
   const int64_t ctas = (f.rows + kRows - 1) / kRows;
-  fn<<<(unsigned)std::min<int64_t>(ctas, (int64_t)sms * std::max(fit, 1)), kCta<TPR>, 0, st>>>(f);
-  return cudaGetLastError();
+  return launch_dependent(fn, dim3((unsigned)std::min<int64_t>(ctas, (int64_t)sms * std::max(fit, 1))), dim3(kCta<TPR>),
+                          0, 1, st, f);
 }
 template <int XT, int ST, int TPR, int VPT>
 cudaError_t run_forward(const Forward& f, int sms, cudaStream_t st) {
