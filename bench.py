@@ -84,6 +84,8 @@ def parse():
     ap.add_argument("--no-arms", action="store_true", help="skip the same-box NCCL and same-model comparison arms")
     ap.add_argument("--bucket-mb", type=float, default=25.0,
                     help="DDP bucket cap in MB for every arm (GPT-2's workload fixes 25)")
+    ap.add_argument("--fused-ops", action="store_true",
+                    help="run the model's norms and feed-forward halves on ops.norm / ops.dense")
     ap.add_argument("--timeline", default="", help="write one step's per-bucket device timeline (JSON) here")
     return ap.parse_args()
 
@@ -288,6 +290,7 @@ def main():
 
         w = GPT2SmallDDP()
         mcfg = GPT2Config.small()
+        mcfg.fused_ops = args.fused_ops
         vocab, mb, seq = mcfg.vocab_size, args.micro_batch or w.micro_batch, args.seq or w.seq
         model_name = "gpt2-small-124M"
     else:
@@ -295,6 +298,7 @@ def main():
 
         w = Llama1BTopK()
         mcfg = LlamaConfig.b1_1()
+        mcfg.fused_ops = args.fused_ops
         vocab, mb, seq = mcfg.vocab_size, args.micro_batch or w.micro_batch, args.seq or w.seq
         model_name = "llama-1.1B"
 
@@ -467,6 +471,8 @@ def main():
             if twoshot_from is not None:
                 out["config"]["twoshot_from_mb"] = None if twoshot_from >= (1 << 60) else twoshot_from / 2 ** 20
         if trainer is not None or arms is not None:
+            if args.fused_ops:
+                out["config"]["fused_ops"] = True
             out["config"]["optimizer_overlap"] = bool(args.hook == "fused" and args.overlap_opt == "on")
             out["config"]["optimizer_in_kernel"] = bool(out["config"]["optimizer_overlap"]
                                                         and args.opt_in_kernel == "on" and args.model == "gpt2")

@@ -21,8 +21,9 @@ struct Forward {
   int64_t ldr;
   const void* w;   // null: no norm, y = x (rows in 8 bits only)
   void* stream;    // [rows, width], written where residual is given
-  void* y;         // [rows, width] of x_type, or e4m3 codes
-  float* scale;    // [rows]: the codes' scales; null: y of x_type
+  void* y;         // [rows, width] of y_type, or e4m3 codes
+  int y_type;      // x_type, or a 16-bit type where x is fp32
+  float* scale;    // [rows]: the codes' scales; null: y of y_type
   float eps;
 };
 cudaError_t forward(const Forward& f, int sms, cudaStream_t st);

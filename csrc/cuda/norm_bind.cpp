@@ -34,14 +34,19 @@ int64_t check_rows(const torch::Tensor& x, const OptTensor& w, const OptTensor& 
 struct Out {
   torch::Tensor y, scale, stream;  // scale only in 8 bits, stream only with a residual
 };
-Out run_forward(const torch::Tensor& x, const OptTensor& weight, double eps, const OptTensor& residual, bool fp8) {
+Out run_forward(const torch::Tensor& x, const OptTensor& weight, double eps, const OptTensor& residual, bool fp8,
+                c10::optional<at::ScalarType> out_dtype) {
   const int64_t width = check_rows(x, weight, residual, eps), rows = x.numel() / width;
+  const auto y_t = fp8 ? at::kFloat8_e4m3fn : out_dtype.has_value() ? *out_dtype : x.scalar_type();
+  TORCH_CHECK(fp8 || y_t == x.scalar_type() || (x.scalar_type() == torch::kFloat32 && is_half(y_t)),
+              "out_dtype must be ", x.scalar_type(), x.scalar_type() == torch::kFloat32 ? ", bfloat16 or float16" : "",
+              "; got ", y_t);
   TORCH_CHECK(weight.has_value() || (fp8 && !residual.has_value()), "weight is needed");
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   if (weight.has_value()) need_cuda(*weight, x, "weight");
   if (residual.has_value()) need_cuda(*residual, x, "residual");
   const c10::cuda::CUDAGuard guard(x.device());
-  auto y = new_cuda(x.sizes(), fp8 ? at::kFloat8_e4m3fn : x.scalar_type(), x);
+  auto y = new_cuda(x.sizes(), y_t, x);
   torch::Tensor scale, stream;
   if (fp8) scale = new_cuda(x.sizes().slice(0, x.dim() - 1), torch::kFloat32, x);
   if (residual.has_value()) stream = new_cuda(x.sizes(), residual->scalar_type(), x);
@@ -66,6 +71,7 @@ Out run_forward(const torch::Tensor& x, const OptTensor& weight, double eps, con
     f.w_type = type_of(w.scalar_type());
   }
   f.y = y.data_ptr();
+  f.y_type = type_of(y_t);
   f.scale = fp8 ? scale.data_ptr<float>() : nullptr;
   f.eps = (float)eps;
   ck(norm::forward(f, sm_count(x.get_device()), at::cuda::getCurrentCUDAStream()), "rms_norm");
@@ -126,8 +132,8 @@ namespace ag = torch::autograd;
 class NormFn : public ag::Function<NormFn> {
  public:
   static ag::variable_list forward(ag::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
-                                   const OptTensor& residual, double eps) {
-    Out o = run_forward(x, weight, eps, residual, false);
+                                   const OptTensor& residual, double eps, c10::optional<at::ScalarType> out_dtype) {
+    Out o = run_forward(x, weight, eps, residual, false, out_dtype);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({residual.has_value() ? o.stream : x, weight});
     ctx->saved_data["eps"] = eps;
@@ -139,26 +145,27 @@ class NormFn : public ag::Function<NormFn> {
     const bool has_r = ctx->saved_data["residual"].toBool();
     const torch::Tensor ds = has_r ? grads[1] : torch::Tensor();
     const torch::Tensor none;
-    if (!grads[0].defined() && !ds.defined()) return {none, none, none, none};
+    if (!grads[0].defined() && !ds.defined()) return {none, none, none, none, none};
     const auto saved = ctx->get_saved_variables();
     const bool nr = has_r && ctx->needs_input_grad(2);
     auto g = gradients(grads[0], ds, saved[0], saved[1], ctx->saved_data["eps"].toDouble(),
                        (at::ScalarType)ctx->saved_data["type"].toInt(), has_r, ctx->needs_input_grad(1));
-    return once({ctx->needs_input_grad(0) ? g[0] : none, g[2], nr ? g[1] : none, none}, "rms_norm");
+    return once({ctx->needs_input_grad(0) ? g[0] : none, g[2], nr ? g[1] : none, none, none}, "rms_norm");
   }
 };
 
 // (y,) or (y, stream).
-std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, double eps, OptTensor residual) {
+std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, double eps, OptTensor residual,
+                                    c10::optional<at::ScalarType> out_dtype) {
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual)))
-    return NormFn::apply(x, weight, residual, eps);
-  Out o = run_forward(x, weight, eps, residual, false);
+    return NormFn::apply(x, weight, residual, eps, out_dtype);
+  Out o = run_forward(x, weight, eps, residual, false, out_dtype);
   if (residual.has_value()) return {o.y, o.stream};
   return {o.y};
 }
 std::vector<torch::Tensor> rms_norm_fp8(torch::Tensor x, OptTensor weight, double eps, OptTensor residual) {
   const at::NoGradGuard no_grad;
-  Out o = run_forward(x, weight, eps, residual, true);
+  Out o = run_forward(x, weight, eps, residual, true, c10::nullopt);
   if (residual.has_value()) return {o.y, o.scale, o.stream};
   return {o.y, o.scale};
 }

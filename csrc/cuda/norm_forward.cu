@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ F
             if (j < valid) p[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
         }
       } else {
-        Raw<XT>::template store<kVec>(f.y, at, valid, v[i]);
+        if (!kVec || valid > 0)
+          put_run<8>(f.y, at, XT == kF32 ? f.y_type : XT, kVec ? 8 : valid, kVec, v[i]);
       }
     }
   }

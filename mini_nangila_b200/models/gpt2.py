@@ -10,6 +10,11 @@ columns and -inf on the padding columns is fused into that GEMM, so the
 padding columns get probability 0 and zero gradient: the loss is the
 cross-entropy over the 50257 real classes and the function computed is
 exactly GPT-2 small's.
+
+``GPT2Config(fused_ops=True)`` runs the blocks' output projections and
+feed-forward halves on ``ops.dense.linear`` (bias, GELU and the residual in the
+products' epilogues): 16-bit operands (a 16-bit model, or ``torch.autocast``),
+CUDA only.
 """
 from __future__ import annotations
 
@@ -18,6 +23,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops import dense
 
 
 @dataclass
@@ -32,6 +39,7 @@ class GPT2Config:
     init_std: float = 0.02
     tie_embeddings: bool = True
     pad_vocab_to: int = 64
+    fused_ops: bool = False
 
     @property
     def padded_vocab(self) -> int:
@@ -54,7 +62,8 @@ class CausalSelfAttention(nn.Module):
         self.c_attn = nn.Linear(cfg.n_embd, 3 * cfg.n_embd)
         self.c_proj = nn.Linear(cfg.n_embd, cfg.n_embd)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def mix(self, x: torch.Tensor) -> torch.Tensor:
+        """The heads' outputs, before the output projection."""
         B, T, C = x.shape
         q, k, v = self.c_attn(x).split(C, dim=2)
         hd = C // self.n_head
@@ -62,7 +71,10 @@ class CausalSelfAttention(nn.Module):
         k = k.view(B, T, self.n_head, hd).transpose(1, 2)
         v = v.view(B, T, self.n_head, hd).transpose(1, 2)
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        return self.c_proj(y.transpose(1, 2).reshape(B, T, C))
+        return y.transpose(1, 2).reshape(B, T, C)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.c_proj(self.mix(x))
 
 
 class MLP(nn.Module):
@@ -82,10 +94,16 @@ class Block(nn.Module):
         self.attn = CausalSelfAttention(cfg)
         self.ln_2 = nn.LayerNorm(cfg.n_embd)
         self.mlp = MLP(cfg)
+        self.fused_ops = cfg.fused_ops
 
     def forward(self, x):
-        x = x + self.attn(self.ln_1(x))
-        return x + self.mlp(self.ln_2(x))
+        if not self.fused_ops:
+            x = x + self.attn(self.ln_1(x))
+            return x + self.mlp(self.ln_2(x))
+        p, fc, out = self.attn.c_proj, self.mlp.c_fc, self.mlp.c_proj
+        x = dense.linear(self.attn.mix(self.ln_1(x)), p.weight, p.bias, residual=x)
+        h = dense.linear(self.ln_2(x), fc.weight, fc.bias, activation="gelu_tanh")
+        return dense.linear(h, out.weight, out.bias, residual=x)
 
 
 class GPT2(nn.Module):

@@ -2,6 +2,12 @@
 grouped-query attention, SwiGLU FFN.  ``LlamaConfig.b1_1()`` is the 1.1B
 configuration (22 layers, d_model 2048, 32 heads, 4 KV heads, FFN 5632,
 vocab 32000, context 2048).
+
+``LlamaConfig(fused_ops=True)`` runs each layer's norms, gated feed-forward
+block and down projection on this framework's kernels (``ops.norm``,
+``ops.dense``): 16-bit operands (a 16-bit model, or ``torch.autocast``), CUDA
+only.  ``Llama.quantize_weights`` then adds an 8-bit form of every projection
+for evaluation under ``torch.no_grad``.
 """
 from __future__ import annotations
 
@@ -10,6 +16,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops import dense, norm
 
 
 @dataclass
@@ -25,6 +33,7 @@ class LlamaConfig:
     rope_theta: float = 10000.0
     eps: float = 1e-5
     init_std: float = 0.02
+    fused_ops: bool = False
 
     @staticmethod
     def b1_1() -> "LlamaConfig":
@@ -44,6 +53,12 @@ class RMSNorm(nn.Module):
     def forward(self, x):
         xf = x.float()
         return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + self.eps)).to(x.dtype) * self.weight
+
+
+def half_type(x: torch.Tensor) -> torch.dtype | None:
+    """The 16-bit type that the fused ops compute in for a float32 stream
+    (autocast's); None where the stream itself has 16 bits."""
+    return torch.get_autocast_dtype("cuda") if x.dtype == torch.float32 and torch.is_autocast_enabled("cuda") else None
 
 
 def rope_tables(seq: int, hd: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -72,14 +87,18 @@ class Attention(nn.Module):
         self.v = nn.Linear(cfg.d_model, cfg.n_kv_head * self.hd, bias=False)
         self.o = nn.Linear(cfg.n_head * self.hd, cfg.d_model, bias=False)
 
-    def forward(self, x, cos, sin):
-        B, T, _ = x.shape
-        q = self.q(x).view(B, T, self.h, self.hd).transpose(1, 2)
-        k = self.k(x).view(B, T, self.kvh, self.hd).transpose(1, 2)
-        v = self.v(x).view(B, T, self.kvh, self.hd).transpose(1, 2)
+    def mix(self, q, k, v, cos, sin):
+        """Attention of the projections [batch, tokens, heads * head_dim]."""
+        B, T, _ = q.shape
+        q = q.view(B, T, self.h, self.hd).transpose(1, 2)
+        k = k.view(B, T, self.kvh, self.hd).transpose(1, 2)
+        v = v.view(B, T, self.kvh, self.hd).transpose(1, 2)
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        return self.o(y.transpose(1, 2).reshape(B, T, self.h * self.hd))
+        return y.transpose(1, 2).reshape(B, T, self.h * self.hd)
+
+    def forward(self, x, cos, sin):
+        return self.o(self.mix(self.q(x), self.k(x), self.v(x), cos, sin))
 
 
 class SwiGLU(nn.Module):
@@ -100,10 +119,39 @@ class Layer(nn.Module):
         self.attn = Attention(cfg)
         self.n2 = RMSNorm(cfg.d_model, cfg.eps)
         self.ffn = SwiGLU(cfg)
+        self.fused_ops = cfg.fused_ops
+        self.w8 = None  # 8-bit weights: {projection: (codes, scale)}
 
     def forward(self, x, cos, sin):
-        x = x + self.attn(self.n1(x), cos, sin)
-        return x + self.ffn(self.n2(x))
+        if not self.fused_ops:
+            x = x + self.attn(self.n1(x), cos, sin)
+            return x + self.ffn(self.n2(x))
+        if self.w8 is not None and not torch.is_grad_enabled():
+            return self._forward_8bit(x, cos, sin)
+        a = self.attn(norm.rms_norm(x, self.n1.weight, self.n1.eps, out_dtype=half_type(x)), cos, sin)
+        n, x = norm.rms_norm(a, self.n2.weight, self.n2.eps, residual=x)
+        h = dense.gated_linear(n, self.ffn.gate.weight, self.ffn.up.weight)
+        return dense.linear(h, self.ffn.down.weight, residual=x)
+
+    def quantize_weights(self) -> None:
+        a, f = self.attn, self.ffn
+        self.w8 = {n: norm.quantize_rows(m.weight) for n, m in
+                   (("q", a.q), ("k", a.k), ("v", a.v), ("o", a.o), ("gate", f.gate), ("up", f.up), ("down", f.down))}
+
+    def _forward_8bit(self, x, cos, sin):
+        t = x.dtype if x.dtype != torch.float32 else half_type(x) or torch.bfloat16
+
+        def project(name, codes, scale, **kw):
+            w, ws = self.w8[name]
+            return dense.linear(codes, w, x_scale=scale, w_scale=ws, **kw)
+
+        n, s = norm.rms_norm_fp8(x, self.n1.weight, self.n1.eps)
+        y = self.attn.mix(*(project(p, n, s, out_dtype=t) for p in "qkv"), cos, sin)
+        a = project("o", *norm.quantize_rows(y), out_dtype=t)
+        n, s, x = norm.rms_norm_fp8(a, self.n2.weight, self.n2.eps, residual=x)
+        (g, gs), (u, us) = self.w8["gate"], self.w8["up"]
+        h = dense.gated_linear(n, g, u, x_scale=s, gate_scale=gs, up_scale=us, out_dtype=t)
+        return project("down", *norm.quantize_rows(h), residual=x)
 
 
 class Llama(nn.Module):
@@ -129,10 +177,23 @@ class Llama(nn.Module):
         x = self.emb(idx)
         for layer in self.layers:
             x = layer(x, cos, sin)
-        logits = self.head(self.norm(x))
+        logits = self.head(norm.rms_norm(x, self.norm.weight, self.norm.eps, out_dtype=half_type(x))
+                           if self.cfg.fused_ops else self.norm(x))
         if targets is None:
             return logits
         return F.cross_entropy(logits.reshape(-1, logits.size(-1)).float(), targets.reshape(-1))
+
+    def quantize_weights(self) -> "Llama":
+        """Lay every layer's projections out in 8 bits (e4m3, one scale an output
+        feature) beside the 16-bit ones; needs ``fused_ops`` and a model on its
+        GPU.  Calls under ``torch.no_grad`` use them from then on; call it again
+        after the weights change."""
+        if not self.cfg.fused_ops:
+            raise ValueError("quantize_weights needs LlamaConfig(fused_ops=True)")
+        with torch.no_grad():
+            for layer in self.layers:
+                layer.quantize_weights()
+        return self
 
     def num_params(self) -> int:
         return sum(p.numel() for p in self.parameters())

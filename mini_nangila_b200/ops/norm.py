@@ -12,16 +12,17 @@ import torch
 from .._ext import cuda
 
 
-def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: torch.Tensor | None = None):
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: torch.Tensor | None = None,
+             out_dtype: torch.dtype | None = None):
     """``s * rsqrt(mean(s^2) + eps) * weight`` over the last dimension.
 
     ``s`` is x, or ``x + residual`` rounded to the residual's type; with a
     residual the call returns ``(y, s)``, s being the stream that goes on.
     x: float32, bfloat16 or float16; residual and weight of x's type or
-    float32; y has x's type.  Gradients reach x, weight and residual, from
-    either output.
+    float32; y has x's type, or a 16-bit ``out_dtype`` where x is float32.
+    Gradients reach x, weight and residual, from either output.
     """
-    out = cuda().rms_norm(x, weight, eps, residual)
+    out = cuda().rms_norm(x, weight, eps, residual, out_dtype)
     return out[0] if residual is None else tuple(out)
 
 
