@@ -469,8 +469,13 @@ torch::Tensor cast(const torch::Tensor& t) {
                                                : at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), t);
 }
 
+int64_t check_act(int64_t act) {
+  TORCH_CHECK(act >= kActNone && act <= kActSilu, "unknown activation");
+  return act;
+}
+
 torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int64_t act, OptTensor residual,
-                     OptTensor x_scale, OptTensor w_scale, c10::optional<at::ScalarType> out_dtype) {
+                     const OptTensor& x_scale, const OptTensor& w_scale, c10::optional<at::ScalarType> out_dtype) {
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     x = cast(x);
     weight = cast(weight);
@@ -490,8 +495,9 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   return linear_forward(x, weight, bias, residual, (int)act, x_scale, w_scale, out_dtype, nullptr);
 }
 
-torch::Tensor gated_linear(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, int64_t act, OptTensor x_scale,
-                           OptTensor gate_scale, OptTensor up_scale, c10::optional<at::ScalarType> out_dtype) {
+torch::Tensor gated_linear(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, int64_t act,
+                           const OptTensor& x_scale, const OptTensor& gate_scale, const OptTensor& up_scale,
+                           c10::optional<at::ScalarType> out_dtype) {
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     x = cast(x);
     w_gate = cast(w_gate);
@@ -531,11 +537,35 @@ std::vector<int64_t> dense_status(int64_t device, bool clear) {
   return {v[0], v[1], v[2], v[3]};
 }
 
+// (x, weight, bias, activation, residual, x_scale, w_scale, out_dtype)
+PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 8, "linear");
+  return THPVariable_Wrap(linear(tensor_arg(a[0], "x"), tensor_arg(a[1], "weight"), opt_tensor_arg(a[2], "bias"),
+                                 check_act(int_arg(a[3])), opt_tensor_arg(a[4], "residual"),
+                                 opt_tensor_arg(a[5], "x_scale"), opt_tensor_arg(a[6], "w_scale"),
+                                 opt_dtype_arg(a[7], "out_dtype")));
+  END_HANDLE_TH_ERRORS
+}
+// (x, w_gate, w_up, activation, x_scale, gate_scale, up_scale, out_dtype)
+PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 8, "gated_linear");
+  return THPVariable_Wrap(gated_linear(tensor_arg(a[0], "x"), tensor_arg(a[1], "w_gate"), tensor_arg(a[2], "w_up"),
+                                       check_act(int_arg(a[3])), opt_tensor_arg(a[4], "x_scale"),
+                                       opt_tensor_arg(a[5], "gate_scale"), opt_tensor_arg(a[6], "up_scale"),
+                                       opt_dtype_arg(a[7], "out_dtype")));
+  END_HANDLE_TH_ERRORS
+}
+PyMethodDef kMethods[] = {
+    {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_linear)), METH_FASTCALL, nullptr},
+    {"gated_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_gated_linear)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 void register_dense(pybind11::module& m) {
-  m.def("linear", &linear);
-  m.def("gated_linear", &gated_linear);
+  if (PyModule_AddFunctions(m.ptr(), kMethods) != 0) throw pybind11::error_already_set();
   m.def("dense_plan", &dense_plan);
   m.def("dense_force_plan", &dense_force_plan);
   m.def("dense_status", &dense_status);

@@ -7,7 +7,10 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include <string>
 
@@ -88,6 +91,41 @@ inline torch::autograd::variable_list once(torch::autograd::variable_list grads,
   for (auto& g : grads)
     if (g.defined()) g = out[i++];
   return grads;
+}
+
+// ---- arguments of the functions that Python calls without pybind: its
+// conversion of eight arguments takes 3 us, half of a call of one token.
+inline const torch::Tensor& tensor_arg(PyObject* o, const char* what) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a torch.Tensor, not ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+inline OptTensor opt_tensor_arg(PyObject* o, const char* what) {
+  if (o == Py_None) return c10::nullopt;
+  return tensor_arg(o, what);
+}
+inline c10::optional<at::ScalarType> opt_dtype_arg(PyObject* o, const char* what) {
+  if (o == Py_None) return c10::nullopt;
+  TORCH_CHECK_TYPE(THPDtype_Check(o), what, " must be a torch.dtype, not ", Py_TYPE(o)->tp_name);
+  return reinterpret_cast<THPDtype*>(o)->scalar_type;
+}
+inline double float_arg(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+inline int64_t int_arg(PyObject* o) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+inline void count_args(Py_ssize_t n, Py_ssize_t want, const char* what) {
+  TORCH_CHECK_TYPE(n == want, what, " takes ", text(want), " arguments");
+}
+inline PyObject* wrap_all(const std::vector<torch::Tensor>& v) {
+  PyObject* t = PyTuple_New((Py_ssize_t)v.size());
+  if (t == nullptr) throw python_error();
+  for (size_t i = 0; i < v.size(); ++i) PyTuple_SET_ITEM(t, (Py_ssize_t)i, THPVariable_Wrap(v[i]));
+  return t;
 }
 
 }  // namespace bind

@@ -155,7 +155,8 @@ class NormFn : public ag::Function<NormFn> {
 };
 
 // (y,) or (y, stream).
-std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, double eps, OptTensor residual,
+std::vector<torch::Tensor> rms_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps,
+                                    const OptTensor& residual,
                                     c10::optional<at::ScalarType> out_dtype) {
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual)))
     return NormFn::apply(x, weight, residual, eps, out_dtype);
@@ -163,16 +164,37 @@ std::vector<torch::Tensor> rms_norm(torch::Tensor x, torch::Tensor weight, doubl
   if (residual.has_value()) return {o.y, o.stream};
   return {o.y};
 }
-std::vector<torch::Tensor> rms_norm_fp8(torch::Tensor x, OptTensor weight, double eps, OptTensor residual) {
+std::vector<torch::Tensor> rms_norm_fp8(const torch::Tensor& x, const OptTensor& weight, double eps,
+                                        const OptTensor& residual) {
   const at::NoGradGuard no_grad;
   Out o = run_forward(x, weight, eps, residual, true, c10::nullopt);
   if (residual.has_value()) return {o.y, o.scale, o.stream};
   return {o.y, o.scale};
 }
 
+// (x, weight, eps, residual, out_dtype)
+PyObject* py_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 5, "rms_norm");
+  return wrap_all(rms_norm(tensor_arg(a[0], "x"), tensor_arg(a[1], "weight"), float_arg(a[2]),
+                           opt_tensor_arg(a[3], "residual"), opt_dtype_arg(a[4], "out_dtype")));
+  END_HANDLE_TH_ERRORS
+}
+// (x, weight or None, eps, residual)
+PyObject* py_rms_norm_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count_args(n, 4, "rms_norm_fp8");
+  return wrap_all(rms_norm_fp8(tensor_arg(a[0], "x"), opt_tensor_arg(a[1], "weight"), float_arg(a[2]),
+                               opt_tensor_arg(a[3], "residual")));
+  END_HANDLE_TH_ERRORS
+}
+PyMethodDef kMethods[] = {
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_rms_norm)), METH_FASTCALL, nullptr},
+    {"rms_norm_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&py_rms_norm_fp8)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 void register_norm(pybind11::module& m) {
-  m.def("rms_norm", &rms_norm);
-  m.def("rms_norm_fp8", &rms_norm_fp8);
+  if (PyModule_AddFunctions(m.ptr(), kMethods) != 0) throw pybind11::error_already_set();
 }

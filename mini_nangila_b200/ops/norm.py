@@ -23,7 +23,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
     Gradients reach x, weight and residual, from either output.
     """
     out = cuda().rms_norm(x, weight, eps, residual, out_dtype)
-    return out[0] if residual is None else tuple(out)
+    return out[0] if residual is None else out
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: torch.Tensor | None = None):
@@ -35,10 +35,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, re
     float8_e4m3fn.  A NaN stays one in its place; an infinity makes its row
     NaN.  No gradient.
     """
-    return tuple(cuda().rms_norm_fp8(x, weight, eps, residual))
+    return cuda().rms_norm_fp8(x, weight, eps, residual)
 
 
 def quantize_rows(x: torch.Tensor):
     """``(codes, scale)`` of the rows of x as ``rms_norm_fp8`` makes them: the
     8-bit form of a weight [out_features, in_features] or of activations."""
-    return tuple(cuda().rms_norm_fp8(x, None, 0.0, None))
+    return cuda().rms_norm_fp8(x, None, 0.0, None)

@@ -99,3 +99,19 @@ def test_quantize_rows_refuses():
     for x, text in ((z(2, 8), "CUDA tensor"), (z(2, 8, dtype=torch.int32), "float32"), (z(2, 0), "1 to 32768")):
         with pytest.raises(RuntimeError, match=text):
             norm.quantize_rows(x)
+
+
+def test_arguments_of_another_kind_are_refused():
+    x, w = z(2, 8), z(3, 8)
+    for call, text in ((lambda: dense.linear(x, 3), "weight must be a torch.Tensor, not int"),
+                       (lambda: dense.linear(x, w, residual=[1]), "residual must be a torch.Tensor"),
+                       (lambda: dense.linear(x, w, out_dtype="bf16"), "out_dtype must be a torch.dtype"),
+                       (lambda: dense.gated_linear(x, w, None), "w_up must be a torch.Tensor"),
+                       (lambda: norm.rms_norm(None, w), "x must be a torch.Tensor"),
+                       (lambda: norm.rms_norm(x, w, residual=0), "residual must be a torch.Tensor"),
+                       (lambda: norm.rms_norm(x, w, "a"), "real number"),
+                       (lambda: norm.quantize_rows([1.0]), "x must be a torch.Tensor")):
+        with pytest.raises(TypeError, match=text):
+            call()
+    with pytest.raises(RuntimeError, match="out_dtype"):
+        norm.rms_norm(z(2, 8), z(8), out_dtype=torch.float32)
