@@ -93,16 +93,27 @@ cudaError_t skinny(const Skinny& g, cudaStream_t s);
 // dy_type; dz null: only db.
 int colsum_parts(int64_t m, int64_t n, int sms);
 cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_t* z_hi, const uint8_t* z_lo, int act,
-                         int half_type, int64_t m, int64_t n, void* dz, float* partial, int parts, void* db,
+                         int half_type, int64_t m, int64_t n, void* dz, int64_t ldd, float* partial, int parts, void* db,
                          cudaStream_t s);
 // out[j] = sum of partial[p, j] over p < parts.
 cudaError_t colsum(const float* partial, int parts, int64_t n, void* out, int type, cudaStream_t s);
 // dg = dh * u * act'(g), du = dh * act(g); z_hi/z_lo[0] hold g, [1] u.
 cudaError_t gated_backward(const void* dh, int64_t ldh, const uint16_t* const z_hi[2], const uint8_t* const z_lo[2],
-                           int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int sms, cudaStream_t s);
-// Rows of `elem`-byte elements copied to a row stride of ldd, the tail zeroed.
-cudaError_t repack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int elem,
-                   cudaStream_t s);
+                           int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int64_t ldd, int sms,
+                           cudaStream_t s);
+// Matrices of `elem`-byte elements copied, up to four in one launch: cols
+// elements a row to a row stride of ldd (a multiple of 128 bytes), the tail zeroed.
+struct Copy {
+  const void* src;
+  int64_t lds;
+  void* dst;
+  int64_t ldd, rows, cols;
+};
+struct Copies {
+  Copy m[4];
+  int n;
+};
+cudaError_t repack(const Copies& c, int elem, cudaStream_t s);
 
 // Status of this device's products: {code, a, b, 0}; see ngl_cuda.cuh.
 cudaError_t read_status(int* out4, bool clear, cudaStream_t s);

@@ -26,12 +26,12 @@ template <int kAct>
 __global__ void __launch_bounds__(kLanesX* kLanesY) k_act_backward(const void* dy, int dy_type, int64_t ldy,
                                                                    const uint16_t* z_hi, const uint8_t* z_lo,
                                                                    int half_type, int64_t m, int64_t n, void* dz,
-                                                                   float* partial) {
+                                                                   int64_t ldd, float* partial) {
   pdl_begin();
   pdl_wait();
   const int64_t col = ((int64_t)blockIdx.x * kLanesX + threadIdx.x) * kColGroup;
   const int valid = (int)max64(0, min64(kColGroup, n - col));
-  const bool vdy = runs_aligned(dy, ldy, type_bytes(dy_type)), vo = runs_aligned(dz, n, 2);
+  const bool vdy = runs_aligned(dy, ldy, type_bytes(dy_type)), vo = runs_aligned(dz, ldd, 2);
   const int64_t ldz = (n + 15) / 16 * 16;
   float sum[kColGroup] = {};
   if (valid > 0) {
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_act_backward(const void* d
           d[j] *= g;
         }
       }
-      if (dz != nullptr) put_run<kColGroup>(dz, r * n + col, half_type, valid, vo, d);
+      if (dz != nullptr) put_run<kColGroup>(dz, r * ldd + col, half_type, valid, vo, d);
 #pragma unroll
       for (int j = 0; j < kColGroup; ++j) sum[j] += d[j];
     }
@@ -94,13 +94,13 @@ template <int kAct>
 __global__ void __launch_bounds__(kLanesX* kLanesY) k_gated_backward(const void* dh, int64_t ldh, const uint16_t* g_hi,
                                                                      const uint8_t* g_lo, const uint16_t* u_hi,
                                                                      const uint8_t* u_lo, int half_type, int64_t m,
-                                                                     int64_t n, void* dg, void* du) {
+                                                                     int64_t n, void* dg, void* du, int64_t ldd) {
   pdl_begin();
   pdl_wait();
   const int64_t col = ((int64_t)blockIdx.x * kLanesX + threadIdx.x) * kColGroup;
   const int valid = (int)max64(0, min64(kColGroup, n - col));
   if (valid <= 0) return;
-  const bool vh = runs_aligned(dh, ldh, 2), vs = runs_aligned(dg, n, 2) && runs_aligned(du, n, 2);
+  const bool vh = runs_aligned(dh, ldh, 2), vs = runs_aligned(dg, ldd, 2) && runs_aligned(du, ldd, 2);
   const int64_t ldz = (n + 15) / 16 * 16;
 #pragma unroll 2
   for (int64_t r = (int64_t)blockIdx.y * kLanesY + threadIdx.y; r < m; r += (int64_t)gridDim.y * kLanesY) {
@@ -115,30 +115,32 @@ __global__ void __launch_bounds__(kLanesX* kLanesY) k_gated_backward(const void*
       a[j] = d[j] * b[j] * s;
       b[j] = d[j] * v;
     }
-    put_run<kColGroup>(dg, r * n + col, half_type, valid, vs, a);
-    put_run<kColGroup>(du, r * n + col, half_type, valid, vs, b);
+    put_run<kColGroup>(dg, r * ldd + col, half_type, valid, vs, a);
+    put_run<kColGroup>(du, r * ldd + col, half_type, valid, vs, b);
   }
 }
 
-// CTA (bx, by): 8 elements a thread of the rows by, by + gridDim.y, ...  The
-// sources come here because their rows are not 16-byte aligned, so loads are
-// single elements (adjacent threads share the sectors through L1); stores are
-// 8 elements wide.
+// CTA (bx, by, bz): 8 elements a thread of the rows by, by + gridDim.y, ... of
+// matrix bz.  The sources come here because their rows are not 16-byte aligned,
+// so loads are single elements (adjacent threads share the sectors through L1);
+// stores are 8 elements wide.
 template <typename T>
-__global__ void __launch_bounds__(256) k_repack(const T* src, int64_t lds, T* dst, int64_t ldd, int64_t rows,
-                                                int64_t cols) {
+__global__ void __launch_bounds__(256) k_repack(const __grid_constant__ Copies all) {
   pdl_begin();
   pdl_wait();
+  const Copy& m = all.m[blockIdx.z];
+  const T* src = static_cast<const T*>(m.src);
+  T* dst = static_cast<T*>(m.dst);
   const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (c >= ldd) return;  // ldd is a multiple of 8
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+  if (c >= m.ldd) return;  // ldd is a multiple of 8
+  for (int64_t r = blockIdx.y; r < m.rows; r += gridDim.y) {
     alignas(16) T v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * lds + c + j] : T(0);
+    for (int j = 0; j < 8; ++j) v[j] = c + j < m.cols ? src[r * m.lds + c + j] : T(0);
     if (sizeof(T) == 2)
-      *reinterpret_cast<uint4*>(dst + r * ldd + c) = *reinterpret_cast<const uint4*>(v);
+      *reinterpret_cast<uint4*>(dst + r * m.ldd + c) = *reinterpret_cast<const uint4*>(v);
     else
-      *reinterpret_cast<uint2*>(dst + r * ldd + c) = *reinterpret_cast<const uint2*>(v);
+      *reinterpret_cast<uint2*>(dst + r * m.ldd + c) = *reinterpret_cast<const uint2*>(v);
   }
 }
 
@@ -168,13 +170,13 @@ cudaError_t colsum(const float* partial, int parts, int64_t n, void* out, int ty
 }
 
 cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_t* z_hi, const uint8_t* z_lo, int act,
-                         int half_type, int64_t m, int64_t n, void* dz, float* partial, int parts, void* db,
+                         int half_type, int64_t m, int64_t n, void* dz, int64_t ldd, float* partial, int parts, void* db,
                          cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)parts);
 #define NGL_CALL(a)                                                                                          \
   e = launch_dependent(&k_act_backward<a>, grid, dim3(kLanesX, kLanesY), 0, 1, s, dy, dy_type, ldy, z_hi, z_lo, \
-                       half_type, m, n, dz, db != nullptr ? partial : nullptr)
+                       half_type, m, n, dz, ldd, db != nullptr ? partial : nullptr)
   cudaError_t e = cudaSuccess;
   NGL_BY_ACT(NGL_CALL)
 #undef NGL_CALL
@@ -182,27 +184,30 @@ cudaError_t act_backward(const void* dy, int dy_type, int64_t ldy, const uint16_
 }
 
 cudaError_t gated_backward(const void* dh, int64_t ldh, const uint16_t* const z_hi[2], const uint8_t* const z_lo[2],
-                           int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int sms, cudaStream_t s) {
+                           int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int64_t ldd, int sms,
+                           cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)row_ctas(m, n, sms));
 #define NGL_CALL(a)                                                                                             \
   e = launch_dependent(&k_gated_backward<a>, grid, dim3(kLanesX, kLanesY), 0, 1, s, dh, ldh, z_hi[0], z_lo[0], \
-                       z_hi[1], z_lo[1], half_type, m, n, dg, du)
+                       z_hi[1], z_lo[1], half_type, m, n, dg, du, ldd)
   cudaError_t e = cudaSuccess;
   NGL_BY_ACT(NGL_CALL)
 #undef NGL_CALL
   return e;
 }
 
-cudaError_t repack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int elem,
-                   cudaStream_t s) {
-  if (rows <= 0 || cols <= 0) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)((ldd + 2047) / 2048), (unsigned)std::min<int64_t>(rows, 65535));
-  if (elem == 1)
-    return launch_dependent(&k_repack<uint8_t>, grid, dim3(256), 0, 1, s, static_cast<const uint8_t*>(src), lds,
-                            static_cast<uint8_t*>(dst), ldd, rows, cols);
-  return launch_dependent(&k_repack<uint16_t>, grid, dim3(256), 0, 1, s, static_cast<const uint16_t*>(src), lds,
-                          static_cast<uint16_t*>(dst), ldd, rows, cols);
+cudaError_t repack(const Copies& c, int elem, cudaStream_t s) {
+  if (c.n <= 0 || c.n > 4) return cudaErrorInvalidValue;
+  int64_t wide = 0, rows = 0;
+  for (int i = 0; i < c.n; ++i) {
+    if (c.m[i].rows <= 0 || c.m[i].cols <= 0) return cudaErrorInvalidValue;
+    wide = std::max(wide, c.m[i].ldd);
+    rows = std::max(rows, c.m[i].rows);
+  }
+  const dim3 grid((unsigned)((wide + 2047) / 2048), (unsigned)std::min<int64_t>(rows, 65535), (unsigned)c.n);
+  return elem == 1 ? launch_dependent(&k_repack<uint8_t>, grid, dim3(256), 0, 1, s, c)
+                   : launch_dependent(&k_repack<uint16_t>, grid, dim3(256), 0, 1, s, c);
 }
 
 }  // namespace dense

@@ -850,8 +850,9 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   // 16 k blocks take about as long as an epilogue with an activation
   const bool busy = args.kb <= 16;
   if (g.type == kE4M3)
-    e = gated ? launch_shape<8, kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
-              : launch_shape<8, kMajorK, kMajorK, true, false>(g, maps, args, sms, s);
+    e = gated  ? launch_shape<8, kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
+        : busy ? launch_shape<16, kMajorK, kMajorK, true, false>(g, maps, args, sms, s)
+               : launch_shape<8, kMajorK, kMajorK, true, false>(g, maps, args, sms, s);
   else if (gated)
     e = launch_shape<8, kMajorK, kMajorK, false, true>(g, maps, args, sms, s);
   else if (g.major_a == kMajorK && g.major_b == kMajorK)

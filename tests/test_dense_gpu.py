@@ -223,3 +223,25 @@ def test_same_bits_again():
         if first is None:
             first = got
         assert all(torch.equal(a, c) for a, c in zip(first, got))
+
+
+@pytest.mark.parametrize("m", [777, 785, 129, 144, 1033])
+def test_last_rows_of_a_ragged_prompt(m):
+    """A few rows behind whole tiles take the few-row kernel where that is
+    quicker: one row's result does not depend on the kernel beyond the bound."""
+    x, w = operands(m, 512, 5632, torch.bfloat16, seed=120)
+    b, r = randn(5632, seed=122, dtype=torch.bfloat16), randn(m, 5632, seed=123, dtype=torch.bfloat16)
+    y, e, z, ez = O.linear(x, w, b, "silu", r)
+    O.close(dense.linear(x, w, b, activation="silu", residual=r), y, e)
+    dy = randn(m, 5632, seed=124, dtype=torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(dense.linear(x, w, b, activation="silu"), leaves, dy)
+    with torch.no_grad():
+        for g, (v, e), name in zip(got, O.linear_grads(dy, x, w, z, ez, "silu", True), "xwb"):
+            O.close(g, v, e, name)
+        h, e, _ = O.gated(x, w, w, "silu")
+        O.close(dense.gated_linear(x, w, w), h, e)
+        x8, xs = norm.quantize_rows(x)
+        w8, ws = norm.quantize_rows(w)
+        y, e, _, _ = O.linear(x8.float(), w8.float(), b, "none", r, out=torch.bfloat16, xs=xs, ws=ws)
+        O.close(dense.linear(x8, w8, b, residual=r, x_scale=xs, w_scale=ws), y, e)
