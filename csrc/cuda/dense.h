@@ -85,7 +85,7 @@ struct Skinny {
   Operand x, w[2];
   Epilogue ep;
 };
-cudaError_t skinny(const Skinny& g, cudaStream_t s);
+cudaError_t skinny(const Skinny& g, int sms, cudaStream_t s);
 
 // ---- elementwise parts of the backward passes
 // dz = dy * act'(z) in half_type (act none: dz = dy, a cast; z is not read),

@@ -127,7 +127,7 @@ void run_skinny(const Shape& sh, const Rows& x, const Rows& w, const Rows* w2, c
   g.w[0] = {w.p(), w.ld};
   if (w2 != nullptr) g.w[1] = {w2->p(), w2->ld};
   g.ep = ep;
-  ck(skinny(g, s), "few-row product");
+  ck(skinny(g, sm_count(x.t.get_device()), s), "few-row product");
 }
 
 // y, and the kept pre-activations in *kept where it is not null.

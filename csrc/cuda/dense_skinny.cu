@@ -2,7 +2,7 @@
 //
 // Mathematics: the epilogue of dense.h over z[i, j] = sum_k x[i, k] w[j, k]
 // for up to 16 rows i.  The rows of x are the 16-row operand of mma m16n8k16
-// and 8 weight rows its 8-column operand; the CTA's 8 warps split k and join
+// and 8 weight rows its 8-column operand; the CTA's warps split k and join
 // their sums in shared memory in warp order.  The sum over k may run in any
 // order as long as both operands agree, so each thread loads 16 contiguous
 // bytes of a row straight into its fragment: no shared memory between the
@@ -21,8 +21,6 @@ namespace dense {
 namespace {
 
 using namespace ngl::dev;
-
-constexpr int kWarps = 8;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, bool bf16) {
@@ -77,8 +75,9 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t v) {
 // consecutive 64-byte blocks of k at a time, all in flight at once.  kHigh: x
 // has more than 8 rows; kVec: rows 16-byte aligned and k a multiple of 16
 // bytes.  Rows beyond the last are read as the last: their sums go nowhere.
-template <int NT, int U, bool kHigh, bool kGated, bool kFp8, bool kVec>
-__global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ Skinny g) {
+// W warps, OCC CTAs an SM.
+template <int W, int OCC, int NT, int U, bool kHigh, bool kGated, bool kFp8, bool kVec>
+__global__ void __launch_bounds__(W * 32, OCC) k_skinny(const __grid_constant__ Skinny g) {
   pdl_begin();
   constexpr int NW = kGated ? 2 : 1;
   constexpr int elem = kFp8 ? 1 : 2;
@@ -115,7 +114,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
                    : "memory");
   }
   pdl_wait();
-  for (int64_t b0 = (int64_t)warp * (U * 64); b0 < kbytes; b0 += kWarps * U * 64) {
+  for (int64_t b0 = (int64_t)warp * (U * 64); b0 < kbytes; b0 += W * U * 64) {
     uint4 wv[U][NW][NT], xa[U], xb[U];
     if (kVec && b0 + U * 64 <= kbytes) {
 #pragma unroll
@@ -190,7 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
 
   // acc[.][n][i]: x row q + 8 (i / 2), weight row 8 n + 2 t + (i & 1)
   constexpr int kX = kHigh ? 16 : 8;
-  __shared__ float part[kWarps][NW][kX][8 * NT + 1];
+  __shared__ float part[W][NW][kX][8 * NT + 1];
 #pragma unroll
   for (int w = 0; w < NW; ++w)
 #pragma unroll
@@ -198,7 +197,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < (kHigh ? 4 : 2); ++i) part[warp][w][q + 8 * (i >> 1)][8 * n + 2 * t + (i & 1)] = acc[w][n][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < kX * 8 * NT; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < kX * 8 * NT; i += W * 32) {
     const int r = i / (8 * NT), c = i % (8 * NT);
     const int64_t row = r, col = j0 + c;
     if (row >= g.m || col >= g.n) continue;
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
     for (int w = 0; w < NW; ++w) {
       s[w] = 0.0f;
 #pragma unroll
-      for (int o = 0; o < kWarps; ++o) s[w] += part[o][w][r][c];
+      for (int o = 0; o < W; ++o) s[w] += part[o][w][r][c];
     }
     const Epilogue& e = g.ep;
     float z = s[0], u = s[NW - 1];
@@ -228,30 +227,36 @@ __global__ void __launch_bounds__(kWarps * 32) k_skinny(const __grid_constant__ 
   }
 }
 
-template <int NT, int U, bool kHigh, bool kGated, bool kFp8>
+template <int W, int OCC, int NT, int U, bool kHigh, bool kGated, bool kFp8>
 cudaError_t launch_nt(const Skinny& g, bool vec, cudaStream_t s) {
   const unsigned grid = (unsigned)((g.n + 8 * NT - 1) / (8 * NT));
-  return launch_dependent(
-      vec ? &k_skinny<NT, U, kHigh, kGated, kFp8, true> : &k_skinny<NT, 2, kHigh, kGated, kFp8, false>, dim3(grid),
-      dim3(kWarps * 32), 0, 1, s, g);
+  return launch_dependent(vec ? &k_skinny<W, OCC, NT, U, kHigh, kGated, kFp8, true>
+                              : &k_skinny<W, OCC, NT, 2, kHigh, kGated, kFp8, false>,
+                          dim3(grid), dim3(W * 32), 0, 1, s, g);
 }
-// 8 loads of weights in flight a thread.
+// With more CTAs than fit at once, small ones that leave room for the next; else
+// 16 warps share a CTA's k, so that its loads go out together.  Times of weights
+// from HBM, 8 warps against 16: 5632 x 2048 6.8 and 8.0 us, 32000 x 2048 28.5 and
+// 34.0 us, gated 2 x 5632 x 2048 9.9 and 12.5 us; 2048 x 5632 8.9 and 6.2 us,
+// gated 2 x 2048 x 768 3.2 and 2.7 us.
 template <bool kGated, bool kFp8>
-cudaError_t launch_skinny(const Skinny& g, bool vec, cudaStream_t s) {
-  if (g.m <= 8)
-    return kGated ? launch_nt<1, 4, false, kGated, kFp8>(g, vec, s) : launch_nt<1, 8, false, kGated, kFp8>(g, vec, s);
-  return kGated ? launch_nt<1, 4, true, kGated, kFp8>(g, vec, s) : launch_nt<2, 4, true, kGated, kFp8>(g, vec, s);
+cudaError_t launch_skinny(const Skinny& g, bool vec, int sms, cudaStream_t s) {
+  if (g.m > 8)
+    return kGated ? launch_nt<8, 2, 1, 4, true, kGated, kFp8>(g, vec, s)
+                  : launch_nt<8, 2, 2, 4, true, kGated, kFp8>(g, vec, s);
+  if ((g.n + 7) / 8 > 2 * sms) return launch_nt<8, 3, 1, kGated ? 4 : 8, false, kGated, kFp8>(g, vec, s);
+  return launch_nt<16, 2, 1, kGated ? 2 : 4, false, kGated, kFp8>(g, vec, s);
 }
 
 }  // namespace
 
-cudaError_t skinny(const Skinny& g, cudaStream_t s) {
+cudaError_t skinny(const Skinny& g, int sms, cudaStream_t s) {
   if (g.m <= 0 || g.m > kSkinnyRows || g.n <= 0 || g.k <= 0) return cudaErrorInvalidValue;
   const int elem = type_bytes(g.type);
   bool vec = (g.k * elem) % 16 == 0 && runs_aligned(g.x.p, g.x.ld, elem) && runs_aligned(g.w[0].p, g.w[0].ld, elem);
   if (g.gated) vec = vec && runs_aligned(g.w[1].p, g.w[1].ld, elem);
-  if (g.type == kE4M3) return g.gated ? launch_skinny<true, true>(g, vec, s) : launch_skinny<false, true>(g, vec, s);
-  return g.gated ? launch_skinny<true, false>(g, vec, s) : launch_skinny<false, false>(g, vec, s);
+  if (g.type == kE4M3) return g.gated ? launch_skinny<true, true>(g, vec, sms, s) : launch_skinny<false, true>(g, vec, sms, s);
+  return g.gated ? launch_skinny<true, false>(g, vec, sms, s) : launch_skinny<false, false>(g, vec, sms, s);
 }
 
 }  // namespace dense
