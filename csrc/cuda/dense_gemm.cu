@@ -45,6 +45,7 @@ struct Args {
   int dual;
   int splits;        // pieces of k of each tile
   uint32_t idesc;
+  uint32_t stage_bytes;  // of TMA's boxes in one stage, both CTAs of a pair
   float* partial;    // [tiles, splits, rows of a tile, NB] sums, where splits > 1
   Epilogue ep;
 };
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
         const CUtensorMap* mb = &maps.b[seg];
         const uint32_t da = base + s * S::kStage, db = da + S::kBytesA;
         if (elect_one()) {
-          if (rank == 0) expect_bytes(full(s), CG * S::kStage);
+          if (rank == 0) expect_bytes(full(s), g.stage_bytes);
           if (MA == kMajorK) {
             tma_load<CG>(da, ma, k, row_a, bar);
           } else {
@@ -827,11 +828,15 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   const int bk = g.type == kE4M3 ? 128 : 64;
   const bool gated = g.dual == kDualN;
   const int tn = gated ? g.nb / 2 : g.nb;
+  // Few rows: a box of 32 rows instead of 128, whose other rows of shared memory
+  // then hold anything; they are rows of the accumulator that nothing reads.
+  // (With 128, fewer than 32 rows took 3 us longer than 32 of them.)
+  const int box_a = g.cg == 1 && g.major_a == kMajorK && g.m <= 32 ? 32 : kRowsA;
   Maps maps;
   std::memset(&maps, 0, sizeof(maps));
   const int na = g.dual == kDualK || g.dual == kDualM ? 2 : 1, nbm = g.dual == kDualK || gated ? 2 : 1;
   for (int i = 0; i < 2; ++i) {
-    if (i < na && !make_map(&maps.a[i], g.a[i], g.type, g.major_a, g.m, g.k, kRowsA))
+    if (i < na && !make_map(&maps.a[i], g.a[i], g.type, g.major_a, g.m, g.k, box_a))
       return cudaErrorInvalidValue;
     if (i < nbm && !make_map(&maps.b[i], g.b[i], g.type, g.major_b, g.n, g.k, gated ? g.nb / 2 : g.nb / g.cg))
       return cudaErrorInvalidValue;
@@ -845,6 +850,7 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.dual = g.dual;
   args.splits = g.splits;
   args.idesc = make_idesc(g);
+  args.stage_bytes = (uint32_t)(g.cg * kBlockBytes * (box_a + g.nb / g.cg));
   args.partial = g.partial;
   args.ep = g.ep;
   // 16 k blocks take about as long as an epilogue with an activation
