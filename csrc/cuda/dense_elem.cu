@@ -144,10 +144,10 @@ __global__ void __launch_bounds__(256) k_repack(const __grid_constant__ Copies a
   }
 }
 
-// Rows of the grid for the 256-column kernels: about 8 CTAs an SM.
-int row_ctas(int64_t m, int64_t n, int sms) {
+// Rows of the grid for the 256-column kernels, for about per_sm CTAs an SM.
+int row_ctas(int64_t m, int64_t n, int sms, int per_sm) {
   const int64_t bx = (n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup);
-  const int64_t want = (int64_t)sms * 8 / std::max<int64_t>(bx, 1);
+  const int64_t want = (int64_t)sms * per_sm / std::max<int64_t>(bx, 1);
   return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 65535), (m + kLanesY - 1) / kLanesY));
 }
 
@@ -162,7 +162,9 @@ int row_ctas(int64_t m, int64_t n, int sms) {
 
 }  // namespace
 
-int colsum_parts(int64_t m, int64_t n, int sms) { return row_ctas(m, n, sms); }
+int colsum_parts(int64_t m, int64_t n, int sms) {
+  return row_ctas(m, n, sms, 5);  // those that fit at once: each writes a row of partial sums
+}
 
 cudaError_t colsum(const float* partial, int parts, int64_t n, void* out, int type, cudaStream_t s) {
   return launch_dependent(&k_colsum, dim3((unsigned)((n + 31) / 32)), dim3(32, kSumY), 0, 1, s, partial, parts, n, out,
@@ -187,7 +189,7 @@ cudaError_t gated_backward(const void* dh, int64_t ldh, const uint16_t* const z_
                            int act, int half_type, int64_t m, int64_t n, void* dg, void* du, int64_t ldd, int sms,
                            cudaStream_t s) {
   if (m <= 0 || n <= 0) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)row_ctas(m, n, sms));
+  const dim3 grid((unsigned)((n + kLanesX * kColGroup - 1) / (kLanesX * kColGroup)), (unsigned)row_ctas(m, n, sms, 8));
 #define NGL_CALL(a)                                                                                             \
   e = launch_dependent(&k_gated_backward<a>, grid, dim3(kLanesX, kLanesY), 0, 1, s, dh, ldh, z_hi[0], z_lo[0], \
                        z_hi[1], z_lo[1], half_type, m, n, dg, du, ldd)

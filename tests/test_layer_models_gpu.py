@@ -8,6 +8,7 @@ import os
 import pytest
 import torch
 
+from mini_nangila_b200 import _ext
 from mini_nangila_b200.models import GPT2, GPT2Config, Llama, LlamaConfig
 from mini_nangila_b200.ops import dense, norm
 from tests import layer_oracle as O
@@ -67,6 +68,7 @@ def test_fused_model_is_as_near_to_fp32_as_the_stock_one(kind, mode):
         assert off[1] <= 2 * off[0] + 2.0 ** -8 * g.norm(), n
 
 
+@pytest.mark.skipif(not _ext.cuda_available(), reason="the CUDA extension is not built")
 @pytest.mark.parametrize("kind", ["gpt2", "llama"])
 def test_fused_model_needs_cuda(kind):
     cfg = GPT2Config.tiny() if kind == "gpt2" else LlamaConfig.tiny()
@@ -326,6 +328,55 @@ def test_outputs_are_ready_for_stock_kernels():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_work_that_forks_and_joins_over_streams(captured):
+    """An operator behind an event of another stream waits for that stream's
+    kernels, stock ones and its own kind, run as they come and from a graph."""
+    w = randn(512, 512, seed=1, std=0.04)
+    big = randn(4096, 512, seed=2)
+    small = randn(4, 512, seed=3)
+    s = randn(512, seed=4)
+    side = torch.cuda.Stream()
+
+    def work(fork):
+        main = torch.cuda.current_stream()
+        a = big
+        for _ in range(4):  # long enough to be running when the other stream starts
+            a = dense.linear(a, w, activation="relu") + 0.25
+        e = torch.cuda.Event()
+        e.record(main)
+        with torch.cuda.stream(side if fork else main):
+            torch.cuda.current_stream().wait_event(e)
+            b = dense.linear(a[-4:], w, residual=small)
+            b = norm.rms_norm(b, s)
+            f = torch.cuda.Event()
+            f.record(torch.cuda.current_stream())
+        c = dense.gated_linear(a, w, w)
+        main.wait_event(f)
+        return dense.linear(b, w, residual=c[-4:]), b, c
+
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        want = work(False)
+        torch.cuda.synchronize()
+        if not captured:
+            for _ in range(10):
+                got = work(True)
+                torch.cuda.synchronize()
+                assert all(torch.equal(p, q) for p, q in zip(got, want))
+            return
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = work(True)
+        for _ in range(10):
+            for t in got:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_autocast_types():
     x, w, b = randn(40, 64, seed=1, dtype=torch.float32), randn(24, 64, seed=2, dtype=torch.float32), \
         randn(24, seed=3, dtype=torch.float32)
@@ -367,8 +418,6 @@ def test_saved_inputs_may_not_change():
 def test_every_plan(cg, nb, splits):
     """Each tile shape, with and without pieces of k, over all operand orders and
     epilogues, at sizes no tile divides."""
-    from mini_nangila_b200 import _ext
-
     m, k, n = 413, 840, 296
     x, w, b = randn(m, k, seed=1), randn(n, k, seed=2, std=k ** -0.5), randn(n, seed=3)
     wu, r, dy = randn(n, k, seed=4, std=k ** -0.5), randn(m, n, seed=5), randn(m, n, seed=6)

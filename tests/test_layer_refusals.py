@@ -3,8 +3,10 @@ any GPU work, so they run here on CPU tensors)."""
 import pytest
 import torch
 
+from mini_nangila_b200 import _ext
 from mini_nangila_b200.ops import dense, norm
 
+pytestmark = pytest.mark.skipif(not _ext.cuda_available(), reason="the CUDA extension is not built")
 BF, F8 = torch.bfloat16, torch.float8_e4m3fn
 
 
