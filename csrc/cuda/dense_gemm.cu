@@ -266,18 +266,20 @@ __device__ __forceinline__ void write_units(const Piece& w, void* out, int64_t l
     if (row < w.rows) *reinterpret_cast<uint4*>(q + (int64_t)i * kRowsAtOnce * ld_bytes) = v;
   }
 }
-// A 16-bit piece of the residual: fetched as it is written, a row's units side by
-// side, so that it can be under way before the sums are ready.
-__device__ __forceinline__ void fetch_units(const Piece& w, const void* src, int64_t ld_bytes, uint4 (&r)[4]) {
-  const int unit = w.lane & 3, r0 = w.lane >> 2;
-  const uint8_t* q = static_cast<const uint8_t*>(src) + (w.row0 + r0) * ld_bytes + (w.col / 8 + unit) * 16;
+// A piece of the residual, 32 rows of 64 bytes (32 columns of 16 bits, or half h
+// of 32 of fp32): fetched as it is written, a row's units side by side, so that
+// it can be under way before the sums are ready.
+__device__ __forceinline__ void fetch_units(const Piece& w, const void* src, int64_t ld_bytes, int unit_cols, int h,
+                                            uint4 (&r)[4]) {
+  const int unit = w.lane & 3, r0 = w.lane >> 2, c = 4 * unit_cols * h + unit * unit_cols;
+  const uint8_t* q =
+      static_cast<const uint8_t*>(src) + (w.row0 + r0) * ld_bytes + (w.col + c) * (int64_t)(16 / unit_cols);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r[i] = unit * 8 < w.cols && i * 8 + r0 < w.rows
-               ? __ldg(reinterpret_cast<const uint4*>(q + (int64_t)i * 8 * ld_bytes))
-               : make_uint4(0, 0, 0, 0);
+    r[i] = c < w.cols && i * 8 + r0 < w.rows ? __ldg(reinterpret_cast<const uint4*>(q + (int64_t)i * 8 * ld_bytes))
+                                             : make_uint4(0, 0, 0, 0);
 }
-__device__ __forceinline__ void add_units(const Piece& w, const uint4 (&r)[4], int type, float (&v)[32]) {
+__device__ __forceinline__ void add_units(const Piece& w, const uint4 (&r)[4], int type, int h, float (&v)[32]) {
   auto at = [&](int row, int unit) { return w.smem + (uint32_t)(row * 4 + (unit ^ ((row >> 1) & 3))) * 16u; };
   const int unit = w.lane & 3, r0 = w.lane >> 2;
   __syncwarp();
@@ -288,12 +290,61 @@ __device__ __forceinline__ void add_units(const Piece& w, const uint4 (&r)[4], i
   for (int c = 0; c < 4; ++c) {
     const uint4 u = lds16(at(w.lane, c));
     const uint32_t p[4] = {u.x, u.y, u.z, u.w};
+    if (type == kF32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float lo, hi;
-      unpack_half2(p[j], type, lo, hi);
-      v[8 * c + 2 * j] += lo;
-      v[8 * c + 2 * j + 1] += hi;
+      for (int j = 0; j < 4; ++j) {
+        if (h == 0) v[4 * c + j] += __uint_as_float(p[j]);
+        else v[16 + 4 * c + j] += __uint_as_float(p[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        unpack_half2(p[j], type, lo, hi);
+        v[8 * c + 2 * j] += lo;
+        v[8 * c + 2 * j + 1] += hi;
+      }
+    }
+  }
+}
+// Staging of 16 fp32 columns of 32 rows for matrices whose rows are not 16-byte
+// aligned: a lane's own row on one side, two rows of 16 adjacent columns on the other.
+__device__ __forceinline__ uint32_t plain_at(const Piece& w, int row, int c) {
+  return w.smem + 4u * (uint32_t)(row * 16 + ((c + (row >> 1)) & 15));
+}
+__device__ __forceinline__ void add_plain(const Piece& w, const void* src, int64_t ld, int type, float (&v)[32]) {
+  const int c = w.lane & 15, sub = w.lane >> 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncwarp();
+    const bool in = 16 * h + c < w.cols;
+    const int64_t first = (w.row0 + sub) * ld + w.col + 16 * h + c;
+    uint32_t t[16];  // all under way before the first is stored
+    if (type == kF32) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        t[i] = in && sub + 2 * i < w.rows ? __ldg(static_cast<const uint32_t*>(src) + first + 2 * i * ld) : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        t[i] = in && sub + 2 * i < w.rows ? __ldg(static_cast<const uint16_t*>(src) + first + 2 * i * ld) : 0u;
+      if (type == kBF16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[i] <<= 16;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[i] = __float_as_uint(half_to_float((uint16_t)t[i], kF16));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(plain_at(w, sub + 2 * i, c)), "r"(t[i]) : "memory");
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float f;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(plain_at(w, w.lane, j)) : "memory");
+      v[16 * h + j] += f;
     }
   }
 }
@@ -312,7 +363,8 @@ __device__ __forceinline__ void write_kept(const Piece& w, uint16_t* hi, uint8_t
   write_units<2>(w, lo, ld, 16, q);
 }
 // `aligned`: rows of out start on 16 bytes (then n is a multiple of a unit).
-// Otherwise a row at a time, a column a lane.
+// Otherwise (kAny) two rows of 16 adjacent columns a store.
+template <bool kAny>
 __device__ __forceinline__ void write_piece(const Piece& w, void* out, int64_t ld, int type, bool aligned,
                                             const float (&v)[32]) {
   if (aligned && type == kF32) {
@@ -328,26 +380,37 @@ __device__ __forceinline__ void write_piece(const Piece& w, void* out, int64_t l
 #pragma unroll
     for (int j = 0; j < 16; ++j) p[j] = pack_half2(v[2 * j], v[2 * j + 1], type);
     write_units<4>(w, out, ld * 2, 8, p);
-  } else {
+  } else if constexpr (kAny) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // 16 columns of 32 rows, two rows a store
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(w.smem + 4 * (w.lane * 16 + ((j + (w.lane >> 1)) & 15))),
-                     "f"(v[16 * h + j])
-                     : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(plain_at(w, w.lane, j)), "f"(v[16 * h + j]) : "memory");
       __syncwarp();
       const int c = w.lane & 15, sub = w.lane >> 4;
       if (16 * h + c < w.cols) {
-#pragma unroll 8
-        for (int r = sub; r < w.rows; r += 2) {
-          float f;
-          asm volatile("ld.shared.f32 %0, [%1];"
-                       : "=f"(f)
-                       : "r"(w.smem + 4 * (r * 16 + ((c + (r >> 1)) & 15)))
-                       : "memory");
-          put(out, (w.row0 + r) * ld + w.col + 16 * h + c, f, type);
+        float t[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(t[i]) : "r"(plain_at(w, sub + 2 * i, c)) : "memory");
+        const int64_t first = (w.row0 + sub) * ld + w.col + 16 * h + c;
+        if (type == kF32) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (sub + 2 * i < w.rows) static_cast<float*>(out)[first + 2 * i * ld] = t[i];
+        } else {
+          uint16_t u[16];
+          if (type == kBF16) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = float_to_half(t[i], kBF16);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[i] = float_to_half(t[i], kF16);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (sub + 2 * i < w.rows) static_cast<uint16_t*>(out)[first + 2 * i * ld] = u[i];
         }
       }
     }
@@ -402,6 +465,8 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
   using S = Shape<CG, NB, EW>;
   constexpr int kBk = kFp8 ? 128 : 64;  // k of one stage
   constexpr int kTileN = kGated ? NB / 2 : NB;
+  // 16 epilogue warps have no registers for unaligned rows: the host knows
+  constexpr bool kAny = EW == 8;
   constexpr int kGroups = kTileN / 32 < EW / 4 ? kTileN / 32 : EW / 4;  // epilogue warps share a tile's columns
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -562,7 +627,9 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     Piece pc;
     pc.smem = base + S::kStages * S::kStage + S::kBarBytes + (uint32_t)(warp - 4) * kStageBytes;
     pc.lane = lane;
-    const bool res_units = !kGated && g.ep.residual != nullptr && g.ep.out_type != kF32 && ev.res && g.n % 8 == 0;
+    const int unit_cols = g.ep.out_type == kF32 ? 4 : 8;  // of the residual in 16 bytes
+    const bool res_units = !kGated && g.ep.residual != nullptr && ev.res && g.n % unit_cols == 0;
+    const int64_t res_ld = g.ep.ldr * (g.ep.out_type == kF32 ? 4 : 2);
     int buf = 0;
     uint32_t bph = 0;
     for (uint32_t w = first; w < items; w += step) {
@@ -579,7 +646,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
       uint4 res[4];
       if (res_units) {
         place(part * kColsW);
-        fetch_units(pc, g.ep.residual, g.ep.ldr * 2, res);
+        fetch_units(pc, g.ep.residual, res_ld, unit_cols, 0, res);
       }
       if (*aborted || !wait_bar(tfull(buf), bph, kWaitNs)) {
         *aborted = 1;
@@ -602,12 +669,12 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
           // this CTA's rows of the slot, all of them: the join looks at the sizes
           Piece q = {pc.smem, (int64_t)((int)rank * kRowsA + quad * 32), c, 32, 32, lane};
           float* p = g.partial + (int64_t)it.part * (CG * kRowsA * NB);
-          write_piece(q, p, NB, kF32, true, v);
+          write_piece<false>(q, p, NB, kF32, true, v);
           if constexpr (kGated) {
             tmem_load32(acc + kTileN + c, v);
             tmem_load_wait();
             q.col += kTileN;
-            write_piece(q, p, NB, kF32, true, v);
+            write_piece<false>(q, p, NB, kF32, true, v);
           }
           continue;
         }
@@ -623,19 +690,23 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= u[j];
         } else {
+          act_run<32>(g.ep.act, v);
           if (res_units) {
-            act_run<32>(g.ep.act, v);
-            add_units(pc, res, g.ep.out_type, v);
+            add_units(pc, res, g.ep.out_type, 0, v);
+            if (g.ep.out_type == kF32) {
+              fetch_units(pc, g.ep.residual, res_ld, unit_cols, 1, res);
+              add_units(pc, res, kF32, 1, v);
+            }
             if (c + 32 < (part + 1) * kColsW) {  // the next piece's, while this one is written
               place(c + 32);
-              fetch_units(pc, g.ep.residual, g.ep.ldr * 2, res);
+              fetch_units(pc, g.ep.residual, res_ld, unit_cols, 0, res);
               place(c);
             }
-          } else {
-            epi_finish<32>(g.ep, ev, inside ? row : 0, col, valid, v);
+          } else if (kAny && g.ep.residual != nullptr) {
+            add_plain(pc, g.ep.residual, g.ep.ldr, g.ep.out_type, v);
           }
         }
-        write_piece(pc, g.ep.out[it.prob], g.ep.ldo, g.ep.out_type, ev.out, v);
+        write_piece<kAny>(pc, g.ep.out[it.prob], g.ep.ldo, g.ep.out_type, ev.out, v);
       }
       fence_before();
       __syncwarp();
@@ -854,7 +925,9 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.partial = g.partial;
   args.ep = g.ep;
   // 16 k blocks take about as long as an epilogue with an activation
-  const bool busy = args.kb <= 16;
+  const int out_bytes = type_bytes(g.ep.out_type);
+  const bool busy = args.kb <= 16 && g.n % (16 / out_bytes) == 0 && runs_aligned(g.ep.out[0], g.ep.ldo, out_bytes) &&
+                    runs_aligned(g.ep.residual, g.ep.ldr, out_bytes);
   if (g.type == kE4M3)
     e = gated  ? launch_shape<8, kMajorK, kMajorK, true, true>(g, maps, args, sms, s)
         : busy ? launch_shape<16, kMajorK, kMajorK, true, false>(g, maps, args, sms, s)

@@ -47,21 +47,26 @@ __device__ __forceinline__ uint4 load_once(const uint8_t* p) {
       : "l"(p));
   return v;
 }
-// The same from any address, zero beyond the row's end.
-template <int elem>
+// The same from any address, zero beyond the row's end: the aligned words that
+// hold its bytes, shifted into place.  Only words with a byte of the row in them
+// are read, so no load leaves the row's first and last word.
 __device__ __forceinline__ uint4 load_any(const uint8_t* row, int64_t at, int64_t k_bytes) {
-  uint32_t w[4] = {0, 0, 0, 0};
-  const uint8_t* q = row + at;
-  if (elem == 2) {
+  const int n = (int)min64(16, k_bytes - at);  // bytes of the row
+  if (n <= 0) return make_uint4(0, 0, 0, 0);
+  const uintptr_t p = reinterpret_cast<uintptr_t>(row + at);
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(p & ~(uintptr_t)3);
+  const int off = (int)(p & 3);
+  uint32_t w[5];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (at + 2 * j < k_bytes) w[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(q)[j] << (16 * (j & 1));
-  } else {
+  for (int j = 0; j < 5; ++j) w[j] = 4 * j < off + n ? __ldg(q + j) : 0u;
+  uint32_t v[4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (at + j < k_bytes) w[j / 4] |= (uint32_t)q[j] << (8 * (j & 3));
+  for (int j = 0; j < 4; ++j) {
+    v[j] = __funnelshift_r(w[j], w[j + 1], 8 * off);
+    const int left = n - 4 * j;  // bytes of this word inside the row
+    v[j] = left >= 4 ? v[j] : left <= 0 ? 0u : v[j] & (0xffffffffu >> (32 - 8 * left));
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // Two e4m3 values as two fp16 (exact).
@@ -140,12 +145,12 @@ __global__ void __launch_bounds__(W * 32, OCC) k_skinny(const __grid_constant__ 
         for (int w = 0; w < NW; ++w)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            wv[u][w][n] = kVec ? (at < kbytes ? load_once(wr[w][n] + at) : none) : load_any<elem>(wr[w][n], at, kbytes);
+            wv[u][w][n] = kVec ? (at < kbytes ? load_once(wr[w][n] + at) : none) : load_any(wr[w][n], at, kbytes);
         xa[u] = kVec ? (at < kbytes ? __ldg(reinterpret_cast<const uint4*>(x0 + at)) : none)
-                     : load_any<elem>(x0, at, kbytes);
+                     : load_any(x0, at, kbytes);
         if (kHigh)
           xb[u] = kVec ? (at < kbytes ? __ldg(reinterpret_cast<const uint4*>(x1 + at)) : none)
-                       : load_any<elem>(x1, at, kbytes);
+                       : load_any(x1, at, kbytes);
       }
     }
 #pragma unroll

@@ -17,7 +17,7 @@ constexpr int kBackCta = TPR < 256 ? 256 : TPR;
 // CTAs of an SM: 128 registers a thread.
 constexpr int back_ctas(int tpr) { return tpr > 256 ? 1 : 2; }
 
-template <int XT, int ST, int TPR, int VPT, bool kVec>
+template <int XT, int ST, int TPR, int VPT, int U>
 __global__ void __launch_bounds__(kBackCta<TPR>, back_ctas(TPR)) k_backward(const __grid_constant__ Backward b) {
   pdl_begin();
   pdl_wait();
@@ -31,22 +31,20 @@ __global__ void __launch_bounds__(kBackCta<TPR>, back_ctas(TPR)) k_backward(cons
   int turn = 0;
   Raw<ST> ns[VPT], ne[VPT];
   Raw<XT> ng[VPT];
-  auto run_of = [&](int i, bool inside) {
-    return inside ? max(0, min(8, width - (i * TPR + t) * 8)) : 0;
-  };
+  constexpr int kStep = TPR * U;  // columns from one unit of a run to the next
   auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int col = (i * TPR + t) * 8, valid = run_of(i, row < b.rows);
-      ns[i].template load<kVec>(b.s, row * b.lds + col, valid);
-      ng[i].template load<kVec>(b.dy, row * b.lddy + col, valid);
-      if (b.ds != nullptr) ne[i].template load<kVec>(b.ds, row * b.ldds + col, valid);
+      const int col = run_col<TPR, U>(i, t), end = row < b.rows ? width : 0;
+      ns[i].template load<U>(b.s, row * b.lds, col, kStep, end);
+      ng[i].template load<U>(b.dy, row * b.lddy, col, kStep, end);
+      if (b.ds != nullptr) ne[i].template load<U>(b.ds, row * b.ldds, col, kStep, end);
     }
   };
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
   fetch(row);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) weight_run(b.w, b.w_type, (i * TPR + t) * 8, width, w[i]);
+  for (int i = 0; i < VPT; ++i) weight_run<U>(b.w, b.w_type, run_col<TPR, U>(i, t), kStep, width, w[i]);
   for (; row < b.rows; row += step) {  // the same for all threads of a group
     Raw<ST> s_now[VPT], e_now[VPT];
     Raw<XT> g_now[VPT];
@@ -74,8 +72,7 @@ __global__ void __launch_bounds__(kBackCta<TPR>, back_ctas(TPR)) k_backward(cons
     const float dot = sum[1] * inv * inv_width;  // mean(dy w hat)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int64_t at = row * b.width + (i * TPR + t) * 8;
-      const int valid = run_of(i, true);
+      const int col = run_col<TPR, U>(i, t);
       float s[8], g[8], e[8] = {};
       s_now[i].to(s);
       g_now[i].to(g);
@@ -86,8 +83,8 @@ __global__ void __launch_bounds__(kBackCta<TPR>, back_ctas(TPR)) k_backward(cons
         dw[i][j] += g[j] * hat;
         e[j] += inv * (g[j] * w[i][j] - hat * dot);
       }
-      Raw<XT>::template store<kVec>(b.dx, at, valid, e);
-      if (b.dres != nullptr) Raw<ST>::template store<kVec>(b.dres, at, valid, e);
+      store_run<U>(b.dx, XT, row * b.width, col, kStep, width, e);
+      if (b.dres != nullptr) store_run<U>(b.dres, ST, row * b.width, col, kStep, width, e);
     }
   }
   if (b.partial == nullptr) return;
@@ -97,33 +94,40 @@ __global__ void __launch_bounds__(kBackCta<TPR>, back_ctas(TPR)) k_backward(cons
       if (group != o) continue;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const int col = (i * TPR + t) * 8;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col + j < width) {
-            if (o > 0) dw[i][j] += dw_sm[col + j];
-            dw_sm[col + j] = dw[i][j];
+        for (int j = 0; j < 8; ++j) {
+          const int c = run_col<TPR, U>(i, t) + (j / U) * kStep + j % U;
+          if (c < width) {
+            if (o > 0) dw[i][j] += dw_sm[c];
+            dw_sm[c] = dw[i][j];
           }
+        }
       }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < width; c += kBackCta<TPR>) b.partial[(int64_t)blockIdx.x * width + c] = dw_sm[c];
   } else {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int col = (i * TPR + t) * 8;
-      put_run<8>(b.partial, (int64_t)blockIdx.x * width + col, kF32, max(0, min(8, width - col)), width % 4 == 0,
-                 dw[i]);
-    }
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = run_col<TPR, U>(i, t) + (j / U) * kStep + j % U;
+        if (c < width) b.partial[(int64_t)blockIdx.x * width + c] = dw[i][j];
+      }
   }
 }
 
 template <int XT, int ST, int TPR, int VPT>
 cudaError_t run_backward(const Backward& b, cudaStream_t st) {
-  const bool vec = b.width % 8 == 0 && runs_aligned(b.dy, b.lddy, type_bytes(XT)) &&
-                   runs_aligned(b.ds, b.ldds, type_bytes(ST)) && runs_aligned(b.s, b.lds, type_bytes(ST)) &&
-                   runs_aligned(b.dx, 0, 1) && runs_aligned(b.dres, 0, 1);
-  auto* fn = vec ? &k_backward<XT, ST, TPR, VPT, true> : &k_backward<XT, ST, TPR, VPT, false>;
+  const Side sides[] = {{b.dy, b.lddy, type_bytes(XT)},
+                        {b.ds, b.ldds, type_bytes(ST)},
+                        {b.s, b.lds, type_bytes(ST)},
+                        {b.dx, b.width, type_bytes(XT)},
+                        {b.dres, b.width, type_bytes(ST)}};
+  const int u = unit_of(b.width, sides);
+  auto* fn = u == 8   ? &k_backward<XT, ST, TPR, VPT, 8>
+             : u == 2 ? &k_backward<XT, ST, TPR, VPT, 2>
+                      : &k_backward<XT, ST, TPR, VPT, 1>;
   // at most 16 KB: several groups only up to rows of 4096 elements
   const int smem = b.partial != nullptr && kBackCta<TPR> / TPR > 1 ? (int)b.width * 4 : 0;
   return launch_dependent(fn, dim3((unsigned)b.parts), dim3(kBackCta<TPR>), smem, 1, st, b);

@@ -70,31 +70,40 @@ __device__ __forceinline__ void row_reduce(float (&v)[N], float* sm, int& turn, 
 template <int T>
 struct Raw {
   uint4 q[T == kF32 ? 2 : 1];
-  // kVec: 8 elements or none, 16-byte aligned; otherwise `valid` of any address.
-  template <bool kVec>
-  __device__ __forceinline__ void load(const void* p, int64_t i, int valid) {
-    if constexpr (kVec) {
-      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (T == kF32 ? 4 : 2));
-      q[0] = valid > 0 ? __ldg(s) : make_uint4(0, 0, 0, 0);
-      if constexpr (T == kF32) q[1] = valid > 0 ? __ldg(s + 1) : make_uint4(0, 0, 0, 0);
+  // The elements of a run lie in units of U adjacent ones: 8 (16 bytes and
+  // more at a time), 2 or 1 where rows are not aligned for more.  c0 is the run's
+  // first column, d the distance from one unit to the next; elements from `end`
+  // on are 0.
+  template <int U>
+  __device__ __forceinline__ void load(const void* p, int64_t row, int c0, int d, int end) {
+    if constexpr (U == 8) {
+      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + (row + c0) * (T == kF32 ? 4 : 2));
+      q[0] = c0 < end ? __ldg(s) : make_uint4(0, 0, 0, 0);
+      if constexpr (T == kF32) q[1] = c0 < end ? __ldg(s + 1) : make_uint4(0, 0, 0, 0);
     } else {
       uint32_t w[8] = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < valid) {
-          if constexpr (T == kF32)
-            w[j] = static_cast<const uint32_t*>(p)[i + j];
-          else
-            w[j / 2] |= (uint32_t)static_cast<const uint16_t*>(p)[i + j] << (16 * (j & 1));
+      for (int j = 0; j < 8; j += U) {
+        const int c = c0 + (j / U) * d;
+        if (c < end) {
+          if constexpr (T == kF32) {
+            if constexpr (U == 2) {
+              const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const float*>(p) + row + c));
+              w[j] = u.x;
+              w[j + 1] = u.y;
+            } else {
+              w[j] = __ldg(static_cast<const uint32_t*>(p) + row + c);
+            }
+          } else if constexpr (U == 2) {
+            w[j / 2] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + row + c));
+          } else {
+            w[j / 2] |= (uint32_t)__ldg(static_cast<const uint16_t*>(p) + row + c) << (16 * (j & 1));
+          }
         }
+      }
       q[0] = make_uint4(w[0], w[1], w[2], w[3]);
       if constexpr (T == kF32) q[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
-  }
-  template <bool kVec>
-  __device__ __forceinline__ static void store(void* p, int64_t i, int valid, const float (&v)[8]) {
-    if (kVec && valid == 0) return;
-    put_run<8>(p, i, T, kVec ? 8 : valid, kVec, v);
   }
   __device__ __forceinline__ void to(float (&v)[8]) const {
     if constexpr (T == kF32) {
@@ -111,9 +120,62 @@ struct Raw {
   }
 };
 
+template <int U>
+__device__ __forceinline__ void store_run(void* p, int type, int64_t row, int c0, int d, int end,
+                                          const float (&v)[8]) {
+  if constexpr (U == 8) {
+    if (c0 < end) put_run<8>(p, row + c0, type, 8, true, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j += U) {
+      const int c = c0 + (j / U) * d;
+      if (c >= end) continue;
+      if (U == 2 && type == kF32)
+        *reinterpret_cast<float2*>(static_cast<float*>(p) + row + c) = make_float2(v[j], v[j + 1]);
+      else if (U == 2)
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p) + row + c) = pack_half2(v[j], v[j + 1], type);
+      else
+        put(p, row + c, v[j], type);
+    }
+  }
+}
+// Columns of thread t's run i: the first, and the distance of its units.
+template <int TPR, int U>
+__device__ __forceinline__ int run_col(int i, int t) {
+  return (i * (8 / U) * TPR + t) * U;
+}
+
 // The weight's run in fp32: the same for every row, so read once a thread.
-__device__ __forceinline__ void weight_run(const void* w, int type, int col, int width, float (&v)[8]) {
-  if (w != nullptr) get_run<8>(w, col, type, max(0, min(8, width - col)), runs_aligned(w, 0, 4), v);
+template <int U>
+__device__ __forceinline__ void weight_run(const void* w, int type, int c0, int d, int width, float (&v)[8]) {
+  if (w == nullptr) return;
+  if constexpr (U == 8) {
+    get_run<8>(w, c0, type, max(0, min(8, width - c0)), runs_aligned(w, 0, 4), v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = c0 + (j / U) * d + j % U;
+      v[j] = c < width ? get(w, c, type) : 0.0f;
+    }
+  }
+}
+
+// Units of a row's elements: 8, 2 or 1 (see Raw::load), from what all matrices allow.
+struct Side {
+  const void* p;
+  int64_t ld;
+  int bytes;
+};
+template <int N>
+int unit_of(int64_t width, const Side (&m)[N]) {
+  int u = width % 8 == 0 ? 8 : width % 2 == 0 ? 2 : 1;
+  for (const Side& s : m) {
+    if (s.p == nullptr) continue;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(s.p) | (uintptr_t)(s.ld * s.bytes);
+    if (u == 8 && a % (s.bytes == 1 ? 8 : 16) != 0) u = 2;
+    if (u == 2 && a % (2 * s.bytes) != 0) u = 1;
+  }
+  return u;
 }
 
 struct Split {

@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
-template <int XT, int ST, int TPR, int VPT, bool kFp8, bool kVec>
+template <int XT, int ST, int TPR, int VPT, bool kFp8, int U>
 __global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ Forward f) {
   pdl_begin();
   pdl_wait();
@@ -31,21 +31,19 @@ __global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ F
   float w[VPT][8];
   Raw<XT> nx[VPT];
   Raw<ST> nr[VPT];
-  auto run_of = [&](int i, bool inside) {
-    return inside ? max(0, min(8, width - (i * TPR + t) * 8)) : 0;
-  };
+  constexpr int kStep = TPR * U;  // columns from one unit of a run to the next
   auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int col = (i * TPR + t) * 8, valid = run_of(i, row < f.rows);
-      nx[i].template load<kVec>(f.x, row * f.ldx + col, valid);
-      if (f.residual != nullptr) nr[i].template load<kVec>(f.residual, row * f.ldr + col, valid);
+      const int col = run_col<TPR, U>(i, t), end = row < f.rows ? width : 0;
+      nx[i].template load<U>(f.x, row * f.ldx, col, kStep, end);
+      if (f.residual != nullptr) nr[i].template load<U>(f.residual, row * f.ldr, col, kStep, end);
     }
   };
   int64_t row = (int64_t)blockIdx.x * kRows + group;
   fetch(row);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) weight_run(f.w, f.w_type, (i * TPR + t) * 8, width, w[i]);
+  for (int i = 0; i < VPT; ++i) weight_run<U>(f.w, f.w_type, run_col<TPR, U>(i, t), kStep, width, w[i]);
   // the loop runs the same number of times for all threads of a CTA
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < f.rows; r0 += step, row += step) {
     const bool inside = row < f.rows;
@@ -66,7 +64,7 @@ __global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ F
             unpack_half2(h, ST, v[i][j], v[i][j + 1]);
           }
         }
-        Raw<ST>::template store<kVec>(f.stream, row * f.width + (i * TPR + t) * 8, run_of(i, inside), v[i]);
+        store_run<U>(f.stream, ST, row * f.width, run_col<TPR, U>(i, t), kStep, inside ? width : 0, v[i]);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[0] += v[i][j] * v[i][j];
@@ -94,31 +92,36 @@ __global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ F
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int64_t at = row * f.width + (i * TPR + t) * 8;
-      const int valid = run_of(i, inside);
+      const int col = run_col<TPR, U>(i, t), end = inside ? width : 0;
       if (kFp8) {
-        const uint32_t lo = e4m3x4(v[i][0] * q, v[i][1] * q, v[i][2] * q, v[i][3] * q);
-        const uint32_t hi = e4m3x4(v[i][4] * q, v[i][5] * q, v[i][6] * q, v[i][7] * q);
-        uint8_t* p = static_cast<uint8_t*>(f.y) + at;
-        if (kVec) {
-          if (valid > 0) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+        const uint32_t b[2] = {e4m3x4(v[i][0] * q, v[i][1] * q, v[i][2] * q, v[i][3] * q),
+                               e4m3x4(v[i][4] * q, v[i][5] * q, v[i][6] * q, v[i][7] * q)};
+        uint8_t* p = static_cast<uint8_t*>(f.y) + row * f.width;
+        if constexpr (U == 8) {
+          if (col < end) *reinterpret_cast<uint2*>(p + col) = make_uint2(b[0], b[1]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < valid) p[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
+          for (int j = 0; j < 8; j += U) {
+            const int c = col + (j / U) * kStep;
+            const uint32_t code = b[j / 4] >> (8 * (j & 3));
+            if (c >= end) continue;
+            if (U == 2)
+              *reinterpret_cast<uint16_t*>(p + c) = (uint16_t)code;
+            else
+              p[c] = (uint8_t)code;
+          }
         }
       } else {
-        if (!kVec || valid > 0)
-          put_run<8>(f.y, at, XT == kF32 ? f.y_type : XT, kVec ? 8 : valid, kVec, v[i]);
+        store_run<U>(f.y, XT == kF32 ? f.y_type : XT, row * f.width, col, kStep, end, v[i]);
       }
     }
   }
 }
 
-template <int XT, int ST, int TPR, int VPT, bool kFp8, bool kVec>
+template <int XT, int ST, int TPR, int VPT, bool kFp8, int U>
 cudaError_t start(const Forward& f, int sms, cudaStream_t st) {
   constexpr int kRows = kCta<TPR> / TPR;
-  auto* fn = &k_forward<XT, ST, TPR, VPT, kFp8, kVec>;
+  auto* fn = &k_forward<XT, ST, TPR, VPT, kFp8, U>;
   static int fit = 0;  // CTAs of an SM, the same on every GPU this is built for
   if (fit == 0) {
     const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, fn, kCta<TPR>, 0);
@@ -130,12 +133,19 @@ cudaError_t start(const Forward& f, int sms, cudaStream_t st) {
 }
 template <int XT, int ST, int TPR, int VPT>
 cudaError_t run_forward(const Forward& f, int sms, cudaStream_t st) {
-  const bool vec = f.width % 8 == 0 && runs_aligned(f.x, f.ldx, type_bytes(XT)) &&
-                   runs_aligned(f.residual, f.ldr, type_bytes(ST)) &&
-                   runs_aligned(f.stream, f.width, type_bytes(ST)) && runs_aligned(f.y, 0, 1);
+  const int bytes = type_bytes(XT);
+  const Side sides[] = {{f.x, f.ldx, bytes},
+                        {f.residual, f.ldr, type_bytes(ST)},
+                        {f.stream, f.width, type_bytes(ST)},
+                        {f.y, f.width, f.scale != nullptr ? 1 : type_bytes(f.y_type)}};
+  const int u = unit_of(f.width, sides);
   if (f.scale != nullptr)
-    return vec ? start<XT, ST, TPR, VPT, true, true>(f, sms, st) : start<XT, ST, TPR, VPT, true, false>(f, sms, st);
-  return vec ? start<XT, ST, TPR, VPT, false, true>(f, sms, st) : start<XT, ST, TPR, VPT, false, false>(f, sms, st);
+    return u == 8   ? start<XT, ST, TPR, VPT, true, 8>(f, sms, st)
+           : u == 2 ? start<XT, ST, TPR, VPT, true, 2>(f, sms, st)
+                    : start<XT, ST, TPR, VPT, true, 1>(f, sms, st);
+  return u == 8   ? start<XT, ST, TPR, VPT, false, 8>(f, sms, st)
+         : u == 2 ? start<XT, ST, TPR, VPT, false, 2>(f, sms, st)
+                  : start<XT, ST, TPR, VPT, false, 1>(f, sms, st);
 }
 template <int XT, int ST>
 cudaError_t forward_of(const Forward& p, int sms, cudaStream_t st) {
