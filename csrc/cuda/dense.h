@@ -1,4 +1,4 @@
-// Dense half of a decoder layer (csrc/cuda/dense_gemm.cu, dense_skinny.cu,
+// Dense half of a decoder layer (csrc/cuda/dense_gemm.cuh, dense_skinny.cu,
 // dense_elem.cu): the matrix product with bias, activation and residual in
 // its epilogue, the gated product of two projections, and their backward
 // passes.  No counterpart in the reference, whose models run stock layers.
