@@ -7,6 +7,7 @@ import os
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from mini_nangila_b200 import _ext
 from mini_nangila_b200.models import GPT2, GPT2Config, Llama, LlamaConfig
@@ -411,6 +412,45 @@ def test_saved_inputs_may_not_change():
         w.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_less_usual_calls():
+    """Views of 8-bit rows, fp32 outputs, expanded and strided vectors, one
+    dimension, inference mode, recomputation, one tensor in two places."""
+    for rows in (5, 60):
+        big, bs = norm.quantize_rows(randn(2 * rows, 160, seed=1))
+        w8, ws = norm.quantize_rows(randn(48, 160, seed=2, std=0.08))
+        for x8, xs, w in ((big[::2], bs[::2], w8), (big[:rows, 3:99], bs[:rows, None], w8[:, 3:99])):
+            y, e, _, _ = O.linear(x8.float(), w.float(), xs=xs.flatten(), ws=ws, out=torch.float32)
+            O.close(dense.linear(x8, w, x_scale=xs, w_scale=ws, out_dtype=torch.float32), y, e)
+        x, w = randn(rows, 96, seed=3), randn(40, 96, seed=4, std=0.1)
+        y, e, _, _ = O.linear(x, w, out=torch.float32)
+        O.close(dense.linear(x, w, out_dtype=torch.float32), y, e)
+        h, e, _ = O.gated(x, w, w, "silu", out=torch.float32)
+        O.close(dense.gated_linear(x, w, w, out_dtype=torch.float32), h, e)
+        b = randn(1, seed=5).expand(40)
+        O.close(dense.linear(x, w, b), *O.linear(x, w, b)[:2])
+        b = randn(80, seed=6)[::2]
+        O.close(dense.linear(x, w, b), *O.linear(x, w, b)[:2])
+        with torch.inference_mode():
+            assert torch.equal(dense.linear(x, w, b), dense.linear(x.clone(), w, b))
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        plain = torch.autograd.grad(dense.gated_linear(xl, wl, wl).sum(), [xl, wl])
+        again = torch.autograd.grad(
+            torch.utils.checkpoint.checkpoint(dense.gated_linear, xl, wl, wl, use_reentrant=False).sum(), [xl, wl])
+        assert all(torch.equal(p, q) for p, q in zip(plain, again))
+        sq = randn(rows, rows, seed=7).requires_grad_()
+        (g,) = torch.autograd.grad(dense.linear(sq, sq).sum(), [sq])
+        v = sq.detach().double()
+        want = v.sum(0)[None].expand(rows, rows)  # of the first operand, and the same of the second
+        bound = 2 * ((rows + 8) * 2.0 ** -23 * v.abs().sum(0)[None] + 2.0 ** -9 * want.abs()) + 2.0 ** -8 * 2 * want.abs()
+        O.close(g, 2 * want, bound.expand(rows, rows) + 1e-30)
+    v = randn(96, seed=8)
+    assert dense.linear(v, w).shape == (40,) and torch.equal(dense.linear(v, w), dense.linear(v[None], w)[0])
+    codes, scale = norm.rms_norm_fp8(v, torch.ones_like(v))
+    assert codes.shape == (96,) and scale.shape == ()
+    assert norm.rms_norm(v, torch.ones_like(v)).shape == (96,)
 
 
 @pytest.mark.gpu
