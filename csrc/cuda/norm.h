@@ -49,7 +49,7 @@ struct Backward {
   float eps;
 };
 int backward_parts(int64_t rows, int64_t width, int sms);
-cudaError_t backward(const Backward& b, int sms, cudaStream_t st);
+cudaError_t backward(const Backward& b, cudaStream_t st);
 
 }  // namespace norm
 }  // namespace ngl

@@ -146,8 +146,7 @@ int backward_parts(int64_t rows, int64_t width, int sms) {
   return (int)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)sms * back_ctas(tpr));
 }
 
-cudaError_t backward(const Backward& b, int sms, cudaStream_t st) {
-  (void)sms;
+cudaError_t backward(const Backward& b, cudaStream_t st) {
   if (b.rows <= 0 || b.width <= 0 || b.width > kMaxWidth) return cudaErrorInvalidValue;
   cudaError_t e;
   if (b.x_type == kF32)

@@ -123,7 +123,7 @@ std::array<torch::Tensor, 3> gradients(const torch::Tensor& dy, const torch::Ten
     b.partial = part.data_ptr<float>();
     b.dw = dw.data_ptr();
   }
-  ck(norm::backward(b, sms, st), "rms_norm backward");
+  ck(norm::backward(b, st), "rms_norm backward");
   return {dx, has_residual ? (split ? dres : dx) : torch::Tensor(), dw};
 }
 

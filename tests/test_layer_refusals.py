@@ -117,3 +117,29 @@ def test_arguments_of_another_kind_are_refused():
             call()
     with pytest.raises(RuntimeError, match="out_dtype"):
         norm.rms_norm(z(2, 8), z(8), out_dtype=torch.float32)
+
+
+def test_plans_of_products():
+    """The planner takes every tile shape somewhere, splits k only where tiles
+    leave SMs idle, and never into pieces of fewer than 4 blocks of k."""
+    plan = _ext.cuda().dense_plan
+    seen = set()
+    for m in (17, 64, 300, 777, 2048, 8192, 100_000):
+        for n in (16, 768, 2048, 5632, 50_304):
+            for k in (64, 771, 2048, 8192):
+                for dual in range(4):
+                    for fp8 in (False, True):
+                        cg, nb, splits = plan(m, n, k, dual, fp8, 148)
+                        assert cg in (1, 2) and nb in (128, 256) and 1 <= splits <= 32
+                        seen.add((cg, nb, splits > 1))
+                        blocks = -(-k // (128 if fp8 else 64)) * (2 if dual == 2 else 1)
+                        tiles = -(-m // (128 * cg)) * -(-n // (nb // 2 if dual == 1 else nb)) * (2 if dual == 3 else 1)
+                        assert splits == 1 or (blocks // splits >= 4 and tiles * splits <= 148 // cg)
+    assert {(c, n) for c, n, _ in seen} == {(1, 128), (1, 256), (2, 128), (2, 256)}
+    assert any(s for *_, s in seen)
+    for bad in ((0, 1, 1, 0, False, 148), (1, 1, 1, 4, False, 148), (1, 1, 1, 0, False, 1)):
+        with pytest.raises(RuntimeError, match="positive"):
+            plan(*bad)
+    for bad in ((3, 128, 1), (1, 64, 1), (1, 128, 0), (2, 256, 65)):
+        with pytest.raises(RuntimeError, match="plan has"):
+            _ext.cuda().dense_force_plan(*bad)
