@@ -178,21 +178,23 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 columns of this warp's 32 lanes.
+// 32 columns of this warp's 32 lanes.  The load and its wait are one statement:
+// nothing may touch the registers between them.
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
   uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
+      : "r"(addr)
+      : "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  A tile with k contiguous
 // has groups of 8 rows 1024 bytes apart; a tile with rows contiguous holds
@@ -673,7 +675,6 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
         const int valid = inside ? pc.cols : 0;
         float v[32];
         tmem_load32(acc + c, v);
-        tmem_load_wait();
         if (it.part >= 0) {
           // this CTA's rows of the slot, all of them: the join looks at the sizes
           Piece q = {pc.smem, (int64_t)((int)rank * kRowsA + quad * 32), c, 32, 32, lane};
@@ -681,7 +682,6 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
           write_piece<false>(q, p, NB, kF32, true, v);
           if constexpr (kGated) {
             tmem_load32(acc + kTileN + c, v);
-            tmem_load_wait();
             q.col += kTileN;
             write_piece<false>(q, p, NB, kF32, true, v);
           }
@@ -693,7 +693,6 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
           float u[32];
           tmem_load32(acc + kTileN + c, u);
           act_run<32>(g.ep.act, v);
-          tmem_load_wait();
           epi_sums<32>(g.ep, ev, 1, inside ? row : 0, col, valid, u);
           if (g.ep.z_hi[1] != nullptr) write_kept(pc, g.ep.z_hi[1], g.ep.z_lo[1], g.ep.ldz, u);
 #pragma unroll
