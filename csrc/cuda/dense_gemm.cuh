@@ -659,7 +659,8 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
         place(part * kColsW);
         fetch_units(pc, g.ep.residual, res_ld, unit_cols, 0, res);
       }
-      if (*aborted || !wait_bar(tfull(buf), bph, kWaitNs)) {
+      // the whole warp's decision: what follows reads tensor memory as a whole warp
+      if (!__all_sync(kFull, *aborted == 0 && wait_bar(tfull(buf), bph, kWaitNs))) {
         *aborted = 1;
         if (lane == 0) set_status(g.status, kTimeoutResult, (int)blockIdx.x, 2);
         break;

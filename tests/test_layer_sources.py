@@ -1,0 +1,38 @@
+"""What the layer kernels' sources have to keep to, read as text: rules whose
+breach could hang the GPU or race, which no run would show for sure."""
+import os
+import re
+
+CUDA = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc", "cuda")
+
+
+def code(name):
+    """The source without comments."""
+    with open(os.path.join(CUDA, name)) as f:
+        text = f.read()
+    return re.sub(r"//[^\n]*|/\*.*?\*/", "", text, flags=re.S)
+
+
+def kernel(text, name):
+    """The body of a __global__ function."""
+    start = text.index("{", text.index(name + "("))
+    depth = 0
+    for i in range(start, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[start:i + 1]
+    raise AssertionError("no end")
+
+
+def test_a_warp_gives_up_as_one():
+    """A wait that runs out is a decision of the whole warp: a warp of which some
+    lanes leave and some go on to the warp-wide loads of tensor memory hangs."""
+    body = kernel(code("dense_gemm.cuh"), "k_gemm")
+    statements = [" ".join(s.split()) for s in re.split(r"[;{}]", body)]
+    waits = [s for s in statements if "wait_bar" in s and "kDrainNs" not in s]
+    assert len(waits) >= 4
+    for s in waits:
+        assert re.search(r"__all_sync\(kFull, .*wait_bar", s), s
+    for s in statements:
+        if re.search(r"\*aborted\b(?! = 1)", s) and "const aborted" not in s:
+            assert "__all_sync(kFull" in s, s
