@@ -573,15 +573,18 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
         }
       }
     }
+    // Until the products have read the last copies: none is in flight into a CTA
+    // that has left.
+    for (int64_t l = loads > S::kStages ? loads - S::kStages : 0; ok && l < loads; ++l)
+      ok = __all_sync(kFull, *aborted == 0 && wait_bar(empty((int)(l % S::kStages)),
+                                                       (uint32_t)((l / S::kStages) & 1), kWaitNs));
     if (!ok) {
       *aborted = 1;
       if (lane == 0) set_status(g.status, kTimeoutCopy, (int)blockIdx.x, 0);
-      // copies in flight land before the shared memory is given up
-      if (rank == 0) {
-        const int64_t from = loads > S::kStages ? loads - S::kStages : 0;
-        for (int64_t l = from; l < loads; ++l)
-          wait_bar(full((int)(l % S::kStages)), (uint32_t)((l / S::kStages) & 1), kDrainNs);
-      }
+      // Products that gave up read no more, so the copies' arrival cannot be waited
+      // for there, nor in a pair at the first CTA's barriers, whose count needs
+      // both CTAs' loads: they have landed long before this has passed.
+      for (const uint64_t t0 = globaltimer(); globaltimer() - t0 < kDrainNs;) __nanosleep(1000);
     }
   } else if (warp == 1 && rank == 0) {
     // ---- products

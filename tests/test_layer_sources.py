@@ -36,3 +36,17 @@ def test_a_warp_gives_up_as_one():
     for s in statements:
         if re.search(r"\*aborted\b(?! = 1)", s) and "const aborted" not in s:
             assert "__all_sync(kFull" in s, s
+
+
+def test_no_copy_outlives_its_cta():
+    """However the loads' warp ends (all copies issued, or a wait given up, its own
+    or another warp's), it leaves only when its copies have landed: it waits for
+    the products that read the last of them, else for a fixed time."""
+    body = kernel(code("dense_gemm.cuh"), "k_gemm")
+    loads = body[body.index("if (warp == 0)"):body.index("else if (warp == 1")]
+    tail = " ".join(loads[loads.index("++loads"):].split())
+    issued = tail.index("wait_bar(empty(")  # behind the loop, over the last kStages loads
+    gave_up = tail.index("if (!ok)")
+    assert issued < gave_up and "loads - S::kStages" in tail[:issued] and "ok = __all_sync" in tail[:issued]
+    assert re.search(r"globaltimer\(\) - t0 < kDrainNs", tail[gave_up:])
+    assert "rank" not in tail  # both CTAs of a pair
