@@ -286,7 +286,7 @@ __device__ __forceinline__ void fetch_units(const Piece& w, const void* src, int
       static_cast<const uint8_t*>(src) + (w.row0 + r0) * ld_bytes + (w.col + c) * (int64_t)(16 / unit_cols);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    r[i] = c < w.cols && i * 8 + r0 < w.rows ? __ldg(reinterpret_cast<const uint4*>(q + (int64_t)i * 8 * ld_bytes))
+    r[i] = c < w.cols && i * 8 + r0 < w.rows ? *reinterpret_cast<const uint4*>(q + (int64_t)i * 8 * ld_bytes)
                                              : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ void add_units(const Piece& w, const uint4 (&r)[4], int type, int h, float (&v)[32]) {
@@ -333,11 +333,11 @@ __device__ __forceinline__ void add_plain(const Piece& w, const void* src, int64
     if (type == kF32) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        t[i] = in && sub + 2 * i < w.rows ? __ldg(static_cast<const uint32_t*>(src) + first + 2 * i * ld) : 0u;
+        t[i] = in && sub + 2 * i < w.rows ? static_cast<const uint32_t*>(src)[first + 2 * i * ld] : 0u;
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        t[i] = in && sub + 2 * i < w.rows ? __ldg(static_cast<const uint16_t*>(src) + first + 2 * i * ld) : 0u;
+        t[i] = in && sub + 2 * i < w.rows ? static_cast<const uint16_t*>(src)[first + 2 * i * ld] : 0u;
       if (type == kBF16) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) t[i] <<= 16;

@@ -204,8 +204,8 @@ __device__ __forceinline__ void put_kept1(uint16_t* hi, uint8_t* lo, int64_t i, 
 // 8 elements from a multiple of 8.  Those behind the row's last are whatever
 // the padding holds: the caller stores none of them.
 __device__ __forceinline__ void get_kept8(const uint16_t* hi, const uint8_t* lo, int64_t i, float (&v)[8]) {
-  const uint4 h = __ldg(reinterpret_cast<const uint4*>(hi + i));
-  const uint2 l = __ldg(reinterpret_cast<const uint2*>(lo + i));
+  const uint4 h = *reinterpret_cast<const uint4*>(hi + i);
+  const uint2 l = *reinterpret_cast<const uint2*>(lo + i);
   const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[2] = {l.x, l.y};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

@@ -44,9 +44,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 // again, do not go through L1.
 __device__ __forceinline__ uint4 load_once(const uint8_t* p) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
   return v;
 }
 // The same from any address, zero beyond the row's end: the aligned words that
@@ -60,7 +61,7 @@ __device__ __forceinline__ uint4 load_any(const uint8_t* row, int64_t at, int64_
   const int off = (int)(p & 3);
   uint32_t w[5];
 #pragma unroll
-  for (int j = 0; j < 5; ++j) w[j] = 4 * j < off + n ? __ldg(q + j) : 0u;
+  for (int j = 0; j < 5; ++j) w[j] = 4 * j < off + n ? q[j] : 0u;
   uint32_t v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -135,8 +136,8 @@ __global__ void __launch_bounds__(W * 32, OCC) k_skinny(const __grid_constant__ 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t at = b0 + u * 64 + t * 16;
-        xa[u] = __ldg(reinterpret_cast<const uint4*>(x0 + at));
-        if (kHigh) xb[u] = __ldg(reinterpret_cast<const uint4*>(x1 + at));
+        xa[u] = *reinterpret_cast<const uint4*>(x0 + at);
+        if (kHigh) xb[u] = *reinterpret_cast<const uint4*>(x1 + at);
       }
     } else {
 #pragma unroll
@@ -148,10 +149,10 @@ __global__ void __launch_bounds__(W * 32, OCC) k_skinny(const __grid_constant__ 
 #pragma unroll
           for (int n = 0; n < NT; ++n)
             wv[u][w][n] = kVec ? (at < kbytes ? load_once(wr[w][n] + at) : none) : load_any(wr[w][n], at, kbytes);
-        xa[u] = kVec ? (at < kbytes ? __ldg(reinterpret_cast<const uint4*>(x0 + at)) : none)
+        xa[u] = kVec ? (at < kbytes ? *reinterpret_cast<const uint4*>(x0 + at) : none)
                      : load_any(x0, at, kbytes);
         if (kHigh)
-          xb[u] = kVec ? (at < kbytes ? __ldg(reinterpret_cast<const uint4*>(x1 + at)) : none)
+          xb[u] = kVec ? (at < kbytes ? *reinterpret_cast<const uint4*>(x1 + at) : none)
                        : load_any(x1, at, kbytes);
       }
     }

@@ -2,7 +2,11 @@
 // may start while the one before it in the stream still runs, sets itself up,
 // and waits (pdl_wait) for its end before it touches any memory that others
 // write.  Saves about 2 us between two calls of few rows.  Every kernel here
-// calls pdl_begin first and pdl_wait in every thread before its first access.
+// calls pdl_begin first and pdl_wait in every thread before its first access, and
+// reads with ordinary loads: the read-only path (__ldg, ld.global.nc) is for
+// memory that nobody writes while the kernel lives, and these live while the
+// kernel in front still writes what they read, weights (an optimizer's step,
+// quantize_rows) like activations.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -80,8 +80,8 @@ struct Raw {
   __device__ __forceinline__ void load(const void* p, int64_t row, int c0, int d, int end) {
     if constexpr (U == 8) {
       const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + (row + c0) * (T == kF32 ? 4 : 2));
-      q[0] = c0 < end ? __ldg(s) : make_uint4(0, 0, 0, 0);
-      if constexpr (T == kF32) q[1] = c0 < end ? __ldg(s + 1) : make_uint4(0, 0, 0, 0);
+      q[0] = c0 < end ? s[0] : make_uint4(0, 0, 0, 0);
+      if constexpr (T == kF32) q[1] = c0 < end ? s[1] : make_uint4(0, 0, 0, 0);
     } else {
       uint32_t w[8] = {};
 #pragma unroll
@@ -90,16 +90,16 @@ struct Raw {
         if (c < end) {
           if constexpr (T == kF32) {
             if constexpr (U == 2) {
-              const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const float*>(p) + row + c));
+              const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const float*>(p) + row + c);
               w[j] = u.x;
               w[j + 1] = u.y;
             } else {
-              w[j] = __ldg(static_cast<const uint32_t*>(p) + row + c);
+              w[j] = static_cast<const uint32_t*>(p)[row + c];
             }
           } else if constexpr (U == 2) {
-            w[j / 2] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + row + c));
+            w[j / 2] = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + row + c);
           } else {
-            w[j / 2] |= (uint32_t)__ldg(static_cast<const uint16_t*>(p) + row + c) << (16 * (j & 1));
+            w[j / 2] |= (uint32_t)static_cast<const uint16_t*>(p)[row + c] << (16 * (j & 1));
           }
         }
       }

@@ -18,8 +18,10 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
+// Rows of more than 16384 elements spill whatever the bound; without the one CTA
+// an SM said aloud, ptxas gave two of these kernels 32 registers a thread.
 template <int XT, int ST, int TPR, int VPT, bool kFp8, int U>
-__global__ void __launch_bounds__(kCta<TPR>) k_forward(const __grid_constant__ Forward f) {
+__global__ void __launch_bounds__(kCta<TPR>, TPR == 512 && VPT == 8) k_forward(const __grid_constant__ Forward f) {
   pdl_begin();
   pdl_wait();
   constexpr int kRows = kCta<TPR> / TPR;

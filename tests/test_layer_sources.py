@@ -50,3 +50,21 @@ def test_no_copy_outlives_its_cta():
     assert issued < gave_up and "loads - S::kStages" in tail[:issued] and "ok = __all_sync" in tail[:issued]
     assert re.search(r"globaltimer\(\) - t0 < kDrainNs", tail[gave_up:])
     assert "rank" not in tail  # both CTAs of a pair
+
+
+def test_dependent_launches_read_with_ordinary_loads():
+    """A programmatic dependent lives while the kernel in front still writes, so
+    nothing may come over the read-only path (its memory must not change while
+    the kernel lives), and no load may move in front of the wait: ordinary loads
+    behind its memory clobber, or volatile asm with one of its own."""
+    names = [n for n in os.listdir(CUDA) if n.startswith(("dense", "norm", "layer"))]
+    assert len(names) > 10
+    for n in names:
+        text = code(n)
+        assert "__ldg" not in text and "__restrict__" not in text, n
+        for m in re.finditer(r"asm\s*(volatile)?\s*\(", text):
+            end = text.index(";\n", m.end())
+            statement = text[m.start():end]
+            assert ".nc" not in statement, (n, statement)
+            if re.search(r"\bld\.global|griddepcontrol", statement):
+                assert m.group(1) and '"memory"' in statement, (n, statement)
