@@ -127,10 +127,13 @@ void force_plan(int cg, int nb, int splits) {
 }
 
 void plan(Gemm& g, int sms, bool may_split) {
+  const int bk = g.type == kE4M3 ? 128 : 64;
+  const int64_t kb = ceil_div(g.k, bk) * (g.dual == kDualK ? 2 : 1);
   if (g_force[0] != 0) {
     g.cg = g_force[0];
     g.nb = g_force[1];
-    g.splits = may_split ? g_force[2] : 1;
+    // at least one k block a piece: a piece without any has no sums to store
+    g.splits = may_split ? (int)std::min<int64_t>(g_force[2], kb) : 1;
     return;
   }
   // Time of a plan = waves of tiles x the longer of their products and their
@@ -145,8 +148,6 @@ void plan(Gemm& g, int sms, bool may_split) {
   // leave most SMs idle.  Splitting the tiles behind
   // the last full wave gained nothing: a busy GPU runs at its power limit, and a
   // wave half empty at a higher clock.
-  const int bk = g.type == kE4M3 ? 128 : 64;
-  const int64_t kb = ceil_div(g.k, bk) * (g.dual == kDualK ? 2 : 1);
   double best = 1e30;
   Gemm c = g;
   for (c.cg = 2; c.cg >= 1; --c.cg)
