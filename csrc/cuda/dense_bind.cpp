@@ -469,6 +469,7 @@ class LinearFn : public ag::Function<LinearFn> {
     return y;
   }
   static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    seen_by_all("the gradient of linear", grads[0]);
     const auto saved = ctx->get_saved_variables();
     const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
     // edges are those of the tensors given, in their order
@@ -490,6 +491,7 @@ class GatedFn : public ag::Function<GatedFn> {
     return h;
   }
   static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list grads) {
+    seen_by_all("the gradient of gated_linear", grads[0]);
     const auto s = ctx->get_saved_variables();
     const bool ng = ctx->needs_input_grad(1), nu = ctx->needs_input_grad(2);
     auto g = gated_gradients(grads[0], s[0], s[1], s[2], s[3], s[4], (int)ctx->saved_data["act"].toInt(),
@@ -511,6 +513,7 @@ int64_t check_act(int64_t act) {
 
 torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int64_t act, OptTensor residual,
                      const OptTensor& x_scale, const OptTensor& w_scale, c10::optional<at::ScalarType> out_dtype) {
+  seen_by_all("linear", x, weight, bias, residual, x_scale, w_scale);
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     x = cast(x);
     weight = cast(weight);
@@ -533,6 +536,7 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
 torch::Tensor gated_linear(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, int64_t act,
                            const OptTensor& x_scale, const OptTensor& gate_scale, const OptTensor& up_scale,
                            c10::optional<at::ScalarType> out_dtype) {
+  seen_by_all("gated_linear", x, w_gate, w_up, x_scale, gate_scale, up_scale);
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     x = cast(x);
     w_gate = cast(w_gate);

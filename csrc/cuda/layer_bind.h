@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <string>
 
@@ -71,6 +72,17 @@ inline Rows rows_of(const torch::Tensor& x, int64_t rows, int64_t cols) {
 
 inline bool wants_grad(const torch::Tensor& t) { return t.requires_grad(); }
 inline bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+
+inline bool has_tangent(const torch::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+inline bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+// The calls here do not go through the dispatcher, so what watches it does not
+// see them: a tangent would be lost without a word, and a trace would hold the
+// output as a constant.
+template <typename... T>
+void seen_by_all(const char* what, const T&... t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), what, " has no forward-mode derivative");
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, " cannot be traced by torch.jit.trace");
+}
 
 // New tensors without the dispatcher's cost (a call of few rows is bound by
 // the host).

@@ -145,6 +145,7 @@ class NormFn : public ag::Function<NormFn> {
     const bool has_r = ctx->saved_data["residual"].toBool();
     const torch::Tensor ds = has_r ? grads[1] : torch::Tensor();
     const torch::Tensor none;
+    seen_by_all("the gradient of rms_norm", grads[0], ds);
     if (!grads[0].defined() && !ds.defined()) return {none, none, none, none, none};
     const auto saved = ctx->get_saved_variables();
     const bool nr = has_r && ctx->needs_input_grad(2);
@@ -158,6 +159,7 @@ class NormFn : public ag::Function<NormFn> {
 std::vector<torch::Tensor> rms_norm(const torch::Tensor& x, const torch::Tensor& weight, double eps,
                                     const OptTensor& residual,
                                     c10::optional<at::ScalarType> out_dtype) {
+  seen_by_all("rms_norm", x, weight, residual);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual)))
     return NormFn::apply(x, weight, residual, eps, out_dtype);
   Out o = run_forward(x, weight, eps, residual, false, out_dtype);
@@ -166,6 +168,7 @@ std::vector<torch::Tensor> rms_norm(const torch::Tensor& x, const torch::Tensor&
 }
 std::vector<torch::Tensor> rms_norm_fp8(const torch::Tensor& x, const OptTensor& weight, double eps,
                                         const OptTensor& residual) {
+  seen_by_all("rms_norm_fp8", x, weight, residual);
   const at::NoGradGuard no_grad;
   Out o = run_forward(x, weight, eps, residual, true, c10::nullopt);
   if (residual.has_value()) return {o.y, o.scale, o.stream};

@@ -10,6 +10,8 @@ Calls run on the current stream of x's device, allocate from PyTorch's
 allocator and can be captured into CUDA graphs.  Under ``torch.autocast`` 16-bit
 operands are made as ``torch.nn.functional.linear`` makes them.  The extension
 must be built, and tensors must be CUDA tensors: there is no PyTorch fallback.
+Forward-mode derivatives and ``torch.jit.trace`` are refused with a
+``NotImplementedError``.
 """
 from __future__ import annotations
 

@@ -3,7 +3,8 @@ a backward pass, and with an output in 8 bits with one scale a row.
 
 Sums and the norm are in fp32.  Rows may have up to 32768 elements.  Tensors
 must be CUDA tensors and the extension must be built: there is no PyTorch
-fallback.
+fallback.  Forward-mode derivatives and ``torch.jit.trace`` are refused with a
+``NotImplementedError``.
 """
 from __future__ import annotations
 
