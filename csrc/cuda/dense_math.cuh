@@ -33,11 +33,12 @@ __device__ __forceinline__ float act_value(float z) {
   return z;
 }
 
-// Value and derivative together.  Beyond |z| = 30 each derivative is 0 or 1
-// to fp32 and the clamp keeps 0 * inf out; a NaN passes.
+// Value and derivative together.  Beyond |z| = 100 the logistic function is 0 or
+// 1 in fp32, and with it each derivative; the clamp keeps 0 * inf out and changes
+// no value.  A NaN passes.
 template <int kAct>
 __device__ __forceinline__ void act_both(float z, float& v, float& d) {
-  const float c = z != z ? z : fminf(fmaxf(z, -30.0f), 30.0f);
+  const float c = z != z ? z : fminf(fmaxf(z, -100.0f), 100.0f);
   if (kAct == kActRelu) {
     v = z < 0.0f ? 0.0f : z;
     d = z != z ? z : (z > 0.0f ? 1.0f : 0.0f);
