@@ -7,7 +7,7 @@ vocab 32000, context 2048).
 block and down projection on this framework's kernels (``ops.norm``,
 ``ops.dense``): 16-bit operands (a 16-bit model, or ``torch.autocast``), CUDA
 only.  ``Llama.quantize_weights`` then adds an 8-bit form of every projection
-for evaluation under ``torch.no_grad``.
+for evaluation: in evaluation mode, under ``torch.no_grad``.
 """
 from __future__ import annotations
 
@@ -59,6 +59,11 @@ def half_type(x: torch.Tensor) -> torch.dtype | None:
     """The 16-bit type that the fused ops compute in for a float32 stream
     (autocast's); None where the stream itself has 16 bits."""
     return torch.get_autocast_dtype("cuda") if x.dtype == torch.float32 and torch.is_autocast_enabled("cuda") else None
+
+
+def _state(w: torch.Tensor) -> tuple[int, int]:
+    """What an update in place or other memory changes (inference tensors count no updates)."""
+    return w.data_ptr(), 0 if w.is_inference() else w._version
 
 
 def rope_tables(seq: int, hd: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -121,12 +126,16 @@ class Layer(nn.Module):
         self.ffn = SwiGLU(cfg)
         self.fused_ops = cfg.fused_ops
         self.w8 = None  # 8-bit weights: {projection: (codes, scale)}
+        self._w8_of = ()  # and the state of the weights that they were made from
 
     def forward(self, x, cos, sin):
         if not self.fused_ops:
             x = x + self.attn(self.n1(x), cos, sin)
             return x + self.ffn(self.n2(x))
-        if self.w8 is not None and not torch.is_grad_enabled():
+        # Not in training, where a recomputed layer runs forward without gradients.
+        if self.w8 is not None and not self.training and not torch.is_grad_enabled():
+            if any(p["weight"] is not w or _state(w) != was for p, w, was in self._w8_of):
+                raise RuntimeError("weights have changed since quantize_weights(); call it again")
             return self._forward_8bit(x, cos, sin)
         a = self.attn(norm.rms_norm(x, self.n1.weight, self.n1.eps, out_dtype=half_type(x)), cos, sin)
         n, x = norm.rms_norm(a, self.n2.weight, self.n2.eps, residual=x)
@@ -135,8 +144,9 @@ class Layer(nn.Module):
 
     def quantize_weights(self) -> None:
         a, f = self.attn, self.ffn
-        self.w8 = {n: norm.quantize_rows(m.weight) for n, m in
-                   (("q", a.q), ("k", a.k), ("v", a.v), ("o", a.o), ("gate", f.gate), ("up", f.up), ("down", f.down))}
+        of = dict(q=a.q, k=a.k, v=a.v, o=a.o, gate=f.gate, up=f.up, down=f.down)
+        self.w8 = {n: norm.quantize_rows(m.weight) for n, m in of.items()}
+        self._w8_of = [(m._parameters, m.weight, _state(m.weight)) for m in of.values()]
 
     def _forward_8bit(self, x, cos, sin):
         t = x.dtype if x.dtype != torch.float32 else half_type(x) or torch.bfloat16
@@ -185,15 +195,17 @@ class Llama(nn.Module):
 
     def quantize_weights(self) -> "Llama":
         """Lay every layer's projections out in 8 bits (e4m3, one scale an output
-        feature) beside the 16-bit ones; needs ``fused_ops`` and a model on its
-        GPU.  Calls under ``torch.no_grad`` use them from then on; call it again
-        after the weights change."""
+        feature) beside the 16-bit ones, and go into evaluation mode; needs
+        ``fused_ops`` and a model on its GPU.  Calls in evaluation mode under
+        ``torch.no_grad`` use them from then on.  Once a weight has changed
+        (an optimizer's step, ``load_state_dict``, another device or type) such
+        calls raise until this is called again."""
         if not self.cfg.fused_ops:
             raise ValueError("quantize_weights needs LlamaConfig(fused_ops=True)")
         with torch.no_grad():
             for layer in self.layers:
                 layer.quantize_weights()
-        return self
+        return self.eval()
 
     def num_params(self) -> int:
         return sum(p.numel() for p in self.parameters())

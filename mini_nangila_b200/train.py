@@ -181,6 +181,8 @@ class BucketAdamW:
         self._pending = None
         hit["t"] += 1
         torch._foreach_add_(hit["steps"], 1)
+        # the kernel writes through addresses, which no tensor's version counts
+        torch.autograd.graph.increment_version(hit["params"])
         self.updated.update(id(p) for p in hit["params"])
 
     def finish_step(self, all_params) -> None:
