@@ -115,8 +115,12 @@ struct Copies {
 };
 cudaError_t repack(const Copies& c, int elem, cudaStream_t s);
 
-// Status of this device's products: {code, a, b, 0}; see ngl_cuda.cuh.
+// Status of the current device's products since it was cleared: {code, CTA, role, 0},
+// the code of ngl_cuda.cuh; waits for stream s.
 cudaError_t read_status(int* out4, bool clear, cudaStream_t s);
+// The copy of those words that kernels write into host memory, or null where no
+// product has been started on the device; reading it waits for nothing.
+int* status_seen(int dev);
 
 }  // namespace dense
 }  // namespace ngl

@@ -41,6 +41,24 @@ class Operands {
   int elem_ = 2;
 };
 
+// An earlier product gave up a wait: what follows would work on an incomplete output.
+struct GaveUp : torch::PyTorchError {
+  using PyTorchError::PyTorchError;
+  PyObject* python_type() override {
+    const pybind11::gil_scoped_acquire gil;
+    return pybind11::module_::import("mini_nangila_b200.ops.dense").attr("DenseError").ptr();  // a class that stays
+  }
+};
+int gave_up(int64_t device) {
+  const volatile int* w = status_seen((int)device);
+  return w == nullptr ? 0 : w[0];
+}
+void check_earlier(const torch::Tensor& x) {
+  if (const int code = gave_up(x.get_device()))
+    throw GaveUp("a dense product on cuda:" + text(x.get_device()) + " gave up a wait (status " + text(code) +
+                 "): its output is incomplete; dense.check() clears the status");
+}
+
 void run_gemm(Gemm& g, const torch::Tensor& like, std::vector<torch::Tensor>& keep, cudaStream_t s) {
   const int sms = sm_count(like.get_device());
   plan(g, sms, true);
@@ -176,6 +194,7 @@ torch::Tensor linear_forward(const torch::Tensor& x, const torch::Tensor& weight
     need_cuda(*x_scale, x, "x_scale");
     need_cuda(*w_scale, x, "w_scale");
   }
+  check_earlier(x);
   const c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   auto y = new_cuda(shape, out_t, x);
@@ -251,6 +270,7 @@ std::array<torch::Tensor, 3> linear_backward(const torch::Tensor& dy, const torc
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   need_cuda(dy, x, "gradient");
   need_cuda(weight, x, "weight");
+  check_earlier(x);
   const c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   torch::Tensor dx, dw, db;
@@ -335,6 +355,7 @@ torch::Tensor gated_forward(const torch::Tensor& x, const torch::Tensor& w_gate,
     need_cuda(*gate_scale, x, "gate_scale");
     need_cuda(*up_scale, x, "up_scale");
   }
+  check_earlier(x);
   const c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   auto h = new_cuda(out_shape(x, sh.n), out_t, x);
@@ -392,6 +413,7 @@ std::array<torch::Tensor, 3> gated_gradients(const torch::Tensor& dh, const torc
   TORCH_CHECK(dh.scalar_type() == x.scalar_type(), "gradient must be ", x.scalar_type(), "; got ", dh.scalar_type());
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (there is no CPU path)");
   need_cuda(dh, x, "gradient");
+  check_earlier(x);
   const c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   torch::Tensor dx, dwg, dwu;
@@ -563,6 +585,13 @@ std::vector<int64_t> dense_plan(int64_t m, int64_t n, int64_t k, int64_t dual, b
   return {g.cg, g.nb, g.splits};
 }
 
+// The words themselves, as a tensor on the CPU (tests write them).
+torch::Tensor dense_status_words(int64_t device) {
+  int* w = status_seen((int)device);
+  TORCH_CHECK(w != nullptr, "no product has run on this device");
+  return torch::from_blob(w, {4}, torch::kInt32);
+}
+
 void dense_force_plan(int64_t cg, int64_t nb, int64_t splits) {
   TORCH_CHECK(cg == 0 || ((cg == 1 || cg == 2) && (nb == 128 || nb == 256) && splits >= 1 && splits <= 64),
               "a plan has 1 or 2 CTAs, 128 or 256 columns, 1 to 64 splits");
@@ -608,4 +637,6 @@ void register_dense(pybind11::module& m) {
   m.def("dense_plan", &dense_plan);
   m.def("dense_force_plan", &dense_force_plan);
   m.def("dense_status", &dense_status);
+  m.def("dense_gave_up", &gave_up);
+  m.def("dense_status_words", &dense_status_words);
 }

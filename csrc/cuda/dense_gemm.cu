@@ -2,7 +2,9 @@
 // join of products whose k is split (dense_gemm.cuh has the kernel).
 #include "dense_gemm.cuh"
 
+#include <atomic>
 #include <cstring>
+#include <mutex>
 
 namespace ngl {
 namespace dense {
@@ -10,20 +12,40 @@ namespace {
 
 __device__ int g_status[4];
 
-// The current device's status words; their address is looked up once a device.
-cudaError_t status_words(int** p) {
-  static int* known[64] = {nullptr};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (known[dev] == nullptr) {
-    void* q = nullptr;
-    e = cudaGetSymbolAddress(&q, g_status);
-    if (e != cudaSuccess) return e;
-    known[dev] = static_cast<int*>(q);
+// A device's status words, and their copy in host memory, which a kernel that
+// gives up writes too: the host sees it at its next call, without asking the GPU.
+struct Words {
+  int* device;
+  int* host;
+};
+constexpr int kMaxDevices = 64;
+Words g_words[kMaxDevices];
+std::atomic<bool> g_words_known[kMaxDevices];
+
+// Those of device dev, the current one; found and allocated once a device.
+cudaError_t status_words(int dev, Words* w) {
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (!g_words_known[dev].load(std::memory_order_acquire)) {
+    static std::mutex m;
+    const std::lock_guard<std::mutex> lock(m);
+    if (!g_words_known[dev].load(std::memory_order_relaxed)) {
+      void *d = nullptr, *h = nullptr;
+      // allowed while a graph is captured: it is no work on a stream
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+      if (e == cudaSuccess) {
+        e = cudaGetSymbolAddress(&d, g_status);
+        if (e == cudaSuccess) e = cudaHostAlloc(&h, 4 * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+        const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e == cudaSuccess) e = back;
+      }
+      if (e != cudaSuccess) return e;
+      std::memset(h, 0, 4 * sizeof(int));
+      g_words[dev] = {static_cast<int*>(d), static_cast<int*>(h)};
+      g_words_known[dev].store(true, std::memory_order_release);
+    }
   }
-  *p = known[dev];
+  *w = g_words[dev];
   return cudaSuccess;
 }
 
@@ -207,8 +229,11 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
   args.stage_bytes = (uint32_t)(g.cg * kBlockBytes * (box_a + g.nb / g.cg));
   args.partial = g.partial;
   args.ep = g.ep;
-  e = status_words(&args.status);
+  Words words;
+  e = status_words(dev, &words);
   if (e != cudaSuccess) return e;
+  args.status = words.device;
+  args.status_host = words.host;
   // 16 k blocks take about as long as an epilogue with an activation
   const int out_bytes = type_bytes(g.ep.out_type);
   Call call;
@@ -237,12 +262,26 @@ cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s) {
 }
 
 cudaError_t read_status(int* out4, bool clear, cudaStream_t s) {
-  int* p = nullptr;
-  cudaError_t e = status_words(&p);
+  int dev = 0;
+  Words w;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = status_words(dev, &w);
   if (e != cudaSuccess) return e;
-  e = cudaMemcpyAsync(out4, p, 4 * sizeof(int), cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess && clear) e = cudaMemsetAsync(p, 0, 4 * sizeof(int), s);
-  return e != cudaSuccess ? e : cudaStreamSynchronize(s);
+  e = cudaMemcpyAsync(out4, w.device, 4 * sizeof(int), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess && clear) e = cudaMemsetAsync(w.device, 0, 4 * sizeof(int), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return e;
+  volatile int* h = w.host;
+  if (out4[0] == 0)
+    for (int i = 0; i < 4; ++i) out4[i] = h[i];
+  if (clear)
+    for (int i = 0; i < 4; ++i) h[i] = 0;
+  return cudaSuccess;
+}
+
+int* status_seen(int dev) {
+  if (dev < 0 || dev >= kMaxDevices || !g_words_known[dev].load(std::memory_order_acquire)) return nullptr;
+  return g_words[dev].host;
 }
 
 }  // namespace dense

@@ -49,6 +49,7 @@ struct Args {
   int mt, nt;        // tiles of one problem along m and n
   int kb;            // k blocks of one operand pair
   int* status;       // this device's status words
+  int* status_host;  // their copy in host memory
   int dual;
   int splits;        // pieces of k of each tile
   uint32_t idesc;
@@ -177,6 +178,19 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Record that a wait ran out, the first since the words were cleared, for
+// check() and, in host memory, for the next call.
+__device__ __forceinline__ void give_up(const Args& g, int code, int role) {
+  if (atomicCAS(g.status, 0, code) != 0) return;
+  g.status[1] = (int)blockIdx.x;
+  g.status[2] = role;
+  volatile int* h = g.status_host;
+  h[1] = (int)blockIdx.x;
+  h[2] = role;
+  __threadfence_system();
+  h[0] = code;
+}
 
 // 32 columns of this warp's 32 lanes.  The load and its wait are one statement:
 // nothing may touch the registers between them.
@@ -580,7 +594,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
                                                        (uint32_t)((l / S::kStages) & 1), kWaitNs));
     if (!ok) {
       *aborted = 1;
-      if (lane == 0) set_status(g.status, kTimeoutCopy, (int)blockIdx.x, 0);
+      if (lane == 0) give_up(g, kTimeoutCopy, 0);
       // Products that gave up read no more, so the copies' arrival cannot be waited
       // for there, nor in a pair at the first CTA's barriers, whose count needs
       // both CTAs' loads: they have landed long before this has passed.
@@ -628,7 +642,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
     }
     if (!ok) {
       *aborted = 1;
-      if (lane == 0) set_status(g.status, kTimeoutPayload, (int)blockIdx.x, 1);
+      if (lane == 0) give_up(g, kTimeoutPayload, 1);
       if (elect_one()) commit<CG>(drained);
       __syncwarp();
       wait_bar(drained, 0, kDrainNs);
@@ -665,7 +679,7 @@ __global__ void __launch_bounds__(128 + 32 * EW, 1) k_gemm(const __grid_constant
       // the whole warp's decision: what follows reads tensor memory as a whole warp
       if (!__all_sync(kFull, *aborted == 0 && wait_bar(tfull(buf), bph, kWaitNs))) {
         *aborted = 1;
-        if (lane == 0) set_status(g.status, kTimeoutResult, (int)blockIdx.x, 2);
+        if (lane == 0) give_up(g, kTimeoutResult, 2);
         break;
       }
       __syncwarp();

@@ -16,6 +16,8 @@ Forward-mode derivatives and ``torch.jit.trace`` are refused with a
 from __future__ import annotations
 
 import torch
+
+from .. import _ext
 from .._ext import cuda
 
 ACTIVATIONS = ("none", "relu", "gelu", "gelu_tanh", "silu")
@@ -23,7 +25,9 @@ _ACT = {a: i for i, a in enumerate(ACTIVATIONS)}
 
 
 class DenseError(RuntimeError):
-    """A product gave up waiting for its own copies; its output is incomplete."""
+    """A product gave up waiting for its own copies; its output is incomplete.
+    Raised by every product on that device from the first one whose call finds
+    it, until ``check`` has reported it."""
 
 
 def _act(activation: str) -> int:
@@ -67,12 +71,25 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *, a
     return cuda().gated_linear(x, w_gate, w_up, _act(activation), x_scale, gate_scale, up_scale, out_dtype)
 
 
+def _index(device: int | torch.device | None) -> int:
+    idx = device.index if isinstance(device, torch.device) else device
+    return torch.cuda.current_device() if idx is None else int(idx)
+
+
 def check(device: int | torch.device | None = None) -> None:
     """Raise ``DenseError`` if a product on ``device`` gave up a wait since the
     last check (waits end after 4 s); synchronises its current stream."""
-    if device is None:
-        device = torch.cuda.current_device()
-    idx = device.index if isinstance(device, torch.device) else int(device)
-    st = cuda().dense_status(torch.cuda.current_device() if idx is None else idx, True)
+    idx = _index(device)
+    st = cuda().dense_status(idx, True)
     if st[0] != 0:
-        raise DenseError(f"dense product failed: device status {st}")
+        raise DenseError(f"a dense product on cuda:{idx} gave up a wait: status {st}")
+
+
+def poll(device: int | torch.device | None = None) -> None:
+    """``check`` without waiting: raise if a product that has ended, of those on
+    ``device``, gave up.  ``check`` clears the status."""
+    ext = _ext._cuda
+    if ext is not None:  # else no product was started
+        idx = _index(device)
+        if code := ext.dense_gave_up(idx):
+            raise DenseError(f"a dense product on cuda:{idx} gave up a wait (status {code})")

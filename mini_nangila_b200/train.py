@@ -28,6 +28,7 @@ from .utils.nvtx import nvtx_range
 import torch.distributed as dist
 from torch.nn.parallel import DistributedDataParallel as DDP
 
+from .ops import dense
 from .parallel.hook import register_nangila_hook
 
 
@@ -234,6 +235,8 @@ class DDPTrainer:
         elif hook != "nccl":
             raise ValueError(f"unknown hook {hook!r}")
         self.steps_done = 0
+        # where the model's dense products run, whose status every step asks for
+        self._products_on = self.device if self.device.type == "cuda" else None
         self.monitor = None
         if monitor:
             from .parallel.monitor import RankMonitor
@@ -272,7 +275,13 @@ class DDPTrainer:
     def model(self) -> torch.nn.Module:
         return self.ddp.module
 
+    def _poll_products(self) -> None:
+        """Raise ``dense.DenseError`` if a product of a step that has ended gave up (waits for nothing)."""
+        if self._products_on is not None:
+            dense.poll(self._products_on)
+
     def step(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+        self._poll_products()
         if self.monitor is not None:
             self.monitor.check(self.steps_done)  # a peer that left is noticed before any launch
         tl = None
@@ -313,7 +322,9 @@ class DDPTrainer:
     def step_host(self, x_host: torch.Tensor, y_host: torch.Tensor) -> float:
         x = x_host.to(self.device, non_blocking=True)
         y = y_host.to(self.device, non_blocking=True)
-        return float(self.step(x, y).item())
+        loss = float(self.step(x, y).item())
+        self._poll_products()
+        return loss
 
     def step_host_async(self, x_host: torch.Tensor, y_host: torch.Tensor):
         """One step from pinned host tensors without waiting for it: the
@@ -348,6 +359,7 @@ class DDPTrainer:
             if pending[1] is not None:
                 pending[1].synchronize()
             losses.append(float(pending[0]))
+        self._poll_products()
         return losses
 
     def fit(self, next_batch, steps: int, log=None, lr: float | None = None, first_step: int = 1) -> list[float]:
@@ -367,6 +379,7 @@ class DDPTrainer:
             loss = self.step(x, y)
             ms = timer.stop_ms()
             losses.append(float(loss))
+            self._poll_products()
             if log is not None:
                 log.row(step, losses[-1], lr, x.numel(), ms)
         return losses
