@@ -33,13 +33,14 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, re
 
     ``codes * scale[..., None]`` is the norm's output: scale (float32, one a
     row) is the row's largest magnitude / 448, at least 2^-126, and codes are
-    float8_e4m3fn.  A NaN stays one in its place; an infinity makes its row
-    NaN.  No gradient.
+    float8_e4m3fn.  A row with a NaN is NaN, one with an infinity NaN there and
+    0 beside it, as in ``rms_norm``.  No gradient.
     """
     return cuda().rms_norm_fp8(x, weight, eps, residual)
 
 
 def quantize_rows(x: torch.Tensor):
     """``(codes, scale)`` of the rows of x as ``rms_norm_fp8`` makes them: the
-    8-bit form of a weight [out_features, in_features] or of activations."""
+    8-bit form of a weight [out_features, in_features] or of activations.  A NaN
+    stays one in its place; an infinity makes ``codes * scale`` of its row NaN."""
     return cuda().rms_norm_fp8(x, None, 0.0, None)
