@@ -71,7 +71,7 @@ void force_plan(int cg, int nb, int splits);
 int64_t partial_floats(const Gemm& g);
 
 // Enqueue the product.  Every operand must be fit for TMA: base 16-byte
-// aligned, row stride a multiple of 16 bytes (ld_fits).  Returns a CUDA
+// aligned, row stride a multiple of 16 bytes.  Returns a CUDA
 // error, or cudaErrorInvalidValue when a tensor map cannot be made.
 cudaError_t gemm(const Gemm& g, int sms, cudaStream_t s);
 

@@ -1,8 +1,12 @@
 // Elementwise parts of the dense backward passes, and repacking of operands
-// whose rows TMA cannot address.  All are bound by HBM bandwidth: each input
-// is read once and each output written once in 16-byte runs.  The gate's
-// gradient of 8192 x 5632 takes 97 us for its 553 MB (5.7 TB/s, 87 % of the
-// copy rate), an activation's of 8192 x 2048 with its column sums 31 us.
+// whose rows TMA cannot address.  Each input is read once and each output
+// written once in 16-byte runs.  The gate's gradient is bound by HBM bandwidth:
+// 8192 x 5632 takes 94 us for its 553 MB (5.9 TB/s, 90 % of the copy rate).  An
+// activation's with its column sums is not: 8192 x 2048 takes 28 us for 117 MB
+// (4.1 TB/s) with 65 % of the issue slots and 40 % of DRAM busy, one wave of five
+// CTAs an SM, whose warps wait for their loads about half of the time.  Two rows
+// of a thread loaded before either is computed took 56 us (94 of the gate's 144):
+// 110 to 128 registers a thread for 48.
 #include "dense.h"
 
 #include <algorithm>

@@ -223,9 +223,12 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
 template <int kMaj>
 constexpr uint32_t kStep = kMaj == kMajorK ? 32u : 2048u;
 
-// EW: warps of the epilogue.  16 where a tile's products take less time than its
-// epilogue (small k: 8192 x 2048 x 256 with GELU and kept z 37 us against 45);
-// else 8, whose registers hold everything.
+// EW: warps of the epilogue.  16 where a tile's products take less time than an
+// epilogue with an activation (up to 16 k blocks), else 8, whose registers hold
+// everything.  16 against 8 warps, bias and GELU: 8192 x 2048 x 256 31 and 33.5 us
+// (with kept z 37 and 45), x 512 33 and 36, 300 x 5632 x 1024 10.5 and 12, 8192 x
+// 2048 x 1024 level at 54; without an epilogue's work 16 warps lose: 14.6 and 13.8,
+// 20.3 and 19.1, 7.9 and 7.5, 36 and 27.5 us.
 template <int CG, int NB, int EW>
 struct Shape {
   static constexpr int kThreads = 128 + 32 * EW;
@@ -754,7 +757,7 @@ template <int CG, int NB, int EW, bool kAny, int MA, int MB, bool kFp8, bool kGa
 cudaError_t launch(const Maps& maps, const Args& args, int sms, cudaStream_t s) {
   using S = Shape<CG, NB, EW>;
   auto* fn = &k_gemm<CG, NB, EW, kAny, MA, MB, kFp8, kGated>;
-  // once a device; setting it again is harmless
+  // holds for the current device alone, so every launch sets it
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t tiles = (int64_t)args.mt * (args.dual == kDualM ? 2 : 1) * args.nt;

@@ -128,7 +128,7 @@ cudaError_t run_backward(const Backward& b, cudaStream_t st) {
   auto* fn = u == 8   ? &k_backward<XT, ST, TPR, VPT, 8>
              : u == 2 ? &k_backward<XT, ST, TPR, VPT, 2>
                       : &k_backward<XT, ST, TPR, VPT, 1>;
-  // at most 16 KB: several groups only up to rows of 4096 elements
+  // at most 8 KB: several groups only up to rows of 2048 elements
   const int smem = b.partial != nullptr && kBackCta<TPR> / TPR > 1 ? (int)b.width * 4 : 0;
   return launch_dependent(fn, dim3((unsigned)b.parts), dim3(kBackCta<TPR>), smem, 1, st, b);
 }

@@ -42,14 +42,14 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
            w_scale: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``activation(x @ weight.T + bias) + residual`` with sums in fp32.
 
-    * ``x``: [..., in_features], bfloat16 or float16; ``weight``: [out_features,
-      in_features] and ``bias``: [out_features] of the same type;
+    * ``x``: [..., in_features], bfloat16 or float16, at least one feature;
+      ``weight``: [out_features, in_features] and ``bias``: [out_features] of the same type;
     * ``residual``: the output's shape, of x's type or float32; the output has
       its type;
     * 8 bits: ``x`` and ``weight`` float8_e4m3fn with ``x_scale`` (one float32 a
       row of x) and ``w_scale`` (one an output feature); bias and output are of
       ``out_dtype`` (bfloat16 by default).  No gradient.
-    * ``out_dtype`` may also be float32.
+    * ``out_dtype`` may also be float32, where no gradient is needed.
 
     The backward pass gives gradients to x, weight, bias and residual.  It
     keeps the sums before an activation in 24 bits, and rounds their gradient
