@@ -134,7 +134,7 @@ class Layer(nn.Module):
             return x + self.ffn(self.n2(x))
         # Not in training, where a recomputed layer runs forward without gradients.
         if self.w8 is not None and not self.training and not torch.is_grad_enabled():
-            if any(p["weight"] is not w or _state(w) != was for p, w, was in self._w8_of):
+            if any(p.get("weight") is not w or _state(w) != was for p, w, was in self._w8_of):
                 raise RuntimeError("weights have changed since quantize_weights(); call it again")
             return self._forward_8bit(x, cos, sin)
         a = self.attn(norm.rms_norm(x, self.n1.weight, self.n1.eps, out_dtype=half_type(x)), cos, sin)
